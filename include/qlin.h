@@ -10,7 +10,7 @@
  * mirrors the reference's `mps.linear(layer, x) -> None` decline
  * (docs/research/2026-10-03-gguf-on-metal.md:117 in roblennon/mac-kernels-public).
  *
- * Dtype codes: 0 f32, 1 f16, 2 bf16, 3 int8, 4 uint8, 5 int32, 6 float8_e4m3fn.
+ * Dtype codes: 0 f32, 1 f16, 2 bf16, 3 int8, 4 uint8, 5 int32, 6 float8_e4m3fn, 7 int64.
  * Shapes: X [m, k] row-major with row pitch ldx elements; Y [m, n] row-major with pitch ldy.
  * Y = X . W^T (+ bias) with W [n, k].
  */
@@ -32,7 +32,7 @@ enum qlin_status {
   QLIN_ETIMEOUT = 4  /* a kernel gave up a bounded wait (reported by qlin_device_status)      */
 };
 
-enum qlin_dtype { QLIN_F32 = 0, QLIN_F16 = 1, QLIN_BF16 = 2, QLIN_I8 = 3, QLIN_U8 = 4, QLIN_I32 = 5, QLIN_E4M3 = 6 };
+enum qlin_dtype { QLIN_F32 = 0, QLIN_F16 = 1, QLIN_BF16 = 2, QLIN_I8 = 3, QLIN_U8 = 4, QLIN_I32 = 5, QLIN_E4M3 = 6, QLIN_I64 = 7 };
 
 /* ggml type ids accepted by the GGUF entry points. */
 enum qlin_gguf_type {
@@ -290,6 +290,71 @@ int qlin_prologue_f16(const void* x, int x_dtype, int64_t m, int64_t k, int64_t 
                       int64_t ldo, int32_t* row_exp, void* stream);
 int qlin_quantize_rows_int8(const void* x, int x_dtype, int64_t m, int64_t k, int64_t ldx, int rotate_group,
                             int perm, int8_t* out, int64_t ldo, float* scale, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Block-scaled 8-bit floating point linear: y = x . W^T (+ bias) with W in e4m3 and one fp32 scale per
+ * block of 128 x 128 (the form in which 8-bit checkpoints store a linear).  No counterpart in the
+ * reference, whose weight formats are the ones above.
+ *   q      e4m3 [n, k] row-major, row pitch ldq bytes (a multiple of 16; k % 16 == 0, 16-byte aligned)
+ *   scale  fp32 [ceil(n / 128), ceil(k / 128)], row pitch ld_scale: W = q * scale of its block
+ * x is brought to e4m3 with one scale per row and block of 128 columns, as qlin_quantize_rows_fp8 does:
+ * in fp32, a = max(max |x|, 2^-100), q_x = e4m3(x * (448 / a)), s_x = a / 448.  Every block's products are
+ * summed in fp32 by the tensor cores and times s_x * scale into the fp32 sum over the blocks; the bias
+ * joins it before the one rounding to y's dtype.  A NaN or an infinity in x makes its row of y non-finite.
+ * x, y, bias f32 / f16 / bf16; k == 0 gives the bias (or zeros).
+ *
+ * qlin_fp8_linear_grad_input: dx = dy . W for the frozen weight as it is stored (no transposed copy);
+ * dy is brought to e4m3 the same way, in blocks of 128 of its n columns.  n == 0 writes zeros.
+ * ------------------------------------------------------------------------------------------ */
+size_t qlin_fp8_linear_workspace(int64_t m, int64_t n, int64_t k);
+int qlin_fp8_linear(const void* x, int x_dtype, int64_t m, int64_t k, int64_t ldx, const void* q, int64_t ldq,
+                    int64_t n, const float* scale, int64_t ld_scale, const void* bias, int bias_dtype, void* y,
+                    int y_dtype, int64_t ldy, void* workspace, size_t workspace_bytes, void* stream);
+size_t qlin_fp8_linear_grad_input_workspace(int64_t m, int64_t n, int64_t k);
+int qlin_fp8_linear_grad_input(const void* dy, int dy_dtype, int64_t m, int64_t n, int64_t lddy, const void* q,
+                               int64_t ldq, int64_t k, const float* scale, int64_t ld_scale, void* dx, int dx_dtype,
+                               int64_t lddx, void* workspace, size_t workspace_bytes, void* stream);
+/* out e4m3 [m, roundup(k, 128)] with row pitch ldo (zeros past column k, rows 8-byte aligned); scale fp32,
+ * block-major: scale[b * ld_scale + row], ld_scale >= m. */
+int qlin_quantize_rows_fp8(const void* x, int x_dtype, int64_t m, int64_t k, int64_t ldx, void* out, int64_t ldo,
+                           float* scale, int64_t ld_scale, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Rotary positions with several axes (time, height, width of image and video tokens), and the RMS norm
+ * of every query and key head with the position rotation in the same pass.  No counterpart in the
+ * reference (its hosts run them as separate framework ops around the quantized linears).
+ *
+ * qlin_rotary_table: positions [tokens, axes] (f32, i32 or i64); axis a turns axes_dim[a] / 2 pairs (host
+ * array, even numbers, at most 256 pairs in all), pair i of it by positions[., a] * theta^(-2 i / axes_dim[a]).
+ * table fp32 [tokens, pairs, 2]: (cos, sin), the axes' pairs one after the other.  The angle is formed
+ * in 64 bits, so the table is right to fp32 rounding at any position.
+ *
+ * qlin_qk_norm_rotary: for each head's row x of head_dim values, v = x * (mean(x^2) + eps)^-1/2 * weight, then
+ * pair i turned by the token's table entry: values (2i, 2i + 1) if interleaved, else (i, i + pairs); values
+ * past 2 * pairs stay v.  q [batch, tokens, q_heads, head_dim] and k alike with k_heads, both of `dtype`, given by
+ * element strides {batch, token, head} and a unit inner stride; outputs alike (they may not overlap the
+ * inputs).  Weights [head_dim] of weight_dtype or NULL (ones).  Table batch stride in floats, 0: one table for
+ * the batch.  All arithmetic in fp32, one rounding to dtype.  head_dim <= 1024; either head count may be 0.
+ *
+ * qlin_qk_norm_rotary_backward: gradients of q, k and of the two weights (weight_dtype, summed in fp32 over
+ * all rows in a fixed order; NULL: not wanted) for the outputs' gradients dq, dk.
+ * ------------------------------------------------------------------------------------------ */
+int qlin_rotary_table(const void* positions, int pos_dtype, int64_t tokens, int axes, const int32_t* axes_dim,
+                      double theta, float* table, void* stream);
+int qlin_qk_norm_rotary(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, int dtype,
+                        int64_t batch, int64_t tokens, int q_heads, int k_heads, int head_dim, const void* q_weight,
+                        const void* k_weight, int weight_dtype, const float* table, int64_t table_batch_stride,
+                        int pairs, float eps, int interleaved, void* q_out, const int64_t* q_out_strides, void* k_out,
+                        const int64_t* k_out_strides, void* stream);
+size_t qlin_qk_norm_rotary_backward_workspace(int64_t batch, int64_t tokens, int q_heads, int k_heads, int head_dim);
+int qlin_qk_norm_rotary_backward(const void* dq, const int64_t* dq_strides, const void* dk, const int64_t* dk_strides,
+                                 const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                                 int dtype, int64_t batch, int64_t tokens, int q_heads, int k_heads, int head_dim,
+                                 const void* q_weight, const void* k_weight, int weight_dtype, const float* table,
+                                 int64_t table_batch_stride, int pairs, float eps, int interleaved, void* q_grad,
+                                 const int64_t* q_grad_strides, void* k_grad, const int64_t* k_grad_strides,
+                                 void* q_weight_grad, void* k_weight_grad, void* workspace, size_t workspace_bytes,
+                                 void* stream);
 
 #ifdef __cplusplus
 }

@@ -345,7 +345,8 @@ const char* qlin_last_error(void) { return g_err; }
 
 int qlin_bounds_check(int reset, uint32_t* count, uint32_t* site, int64_t* index, int64_t* limit, uint32_t* block) {
   int (*const readers[])(BoundsRecord*, int) = {bounds_read_api, bounds_read_aux,  bounds_read_f16, bounds_read_f16_blk,
-                                                bounds_read_f16_kq, bounds_read_gemv, bounds_read_i8};
+                                                bounds_read_f16_kq, bounds_read_gemv, bounds_read_i8,
+                                                bounds_read_fp8, bounds_read_rotary};
   uint32_t total = 0;
   BoundsRecord first{};
   for (auto rd : readers) {

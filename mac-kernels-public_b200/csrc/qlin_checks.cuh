@@ -53,6 +53,13 @@ enum BoundsSite : unsigned int {
   BS_GRAD = 23,           // gradient prologue / transpose / rotation kernels
   BS_KITCHEN = 24,        // kitchen int8 grid kernel
   BS_PEER_FLAG = 25,      // peer flag words
+  BS_FP8_QUANT = 26,      // fp8 row quantizer: input, codes, scales
+  BS_FP8_SCALE = 27,      // fp8 GEMM block scales, bias
+  BS_FP8_Y = 28,          // fp8 GEMM output element
+  BS_FP8_SMEM = 29,       // fp8 GEMM shared-memory layout
+  BS_FP8_X = 30,          // fp8 small-M kernel: activation read
+  BS_ROT_IN = 31,         // rotary / head norm kernels: input, weight, table
+  BS_ROT_OUT = 32,        // rotary / head norm kernels: output, gradient partials
 };
 
 #ifdef QLIN_CHECKS

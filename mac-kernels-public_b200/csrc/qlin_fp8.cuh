@@ -1,0 +1,345 @@
+// Block-scaled 8-bit linear on the tensor cores (tcgen05.mma kind::f8f6f4, fp32 accumulation).
+//
+//   Y[m, n] = sum_b sx[b][m] * S[n / 128][b] * P_b[m, n]  (+ bias[n]),
+//   P_b[m, n] = sum_{d in block b of 128} xq[m, d] * W[n, d]
+//
+// xq are the activations in e4m3 with one scale per row and block (the row quantizer below), W the
+// stored e4m3 weight with one scale S per 128 x 128 block.  The input gradient is the same sum with the
+// weight's rows as the contraction (kTrans): W is then read as it lies, as a transposed operand.
+//
+// The scales change with every block, so each block's products go to a TMEM buffer of their own and
+// the epilogue warps fold them into fp32 registers, one packed FMA per two values, while the tensor
+// cores fill the next buffer.  Tokens lie on the TMEM lanes: a thread owns one token, whose scale times
+// the warp's block scale is one factor for all of its values.
+//
+// Warp roles (320 threads, one CTA per SM, persistent over the tiles):
+//   warp 0        TMA producer            warp 1   TMEM alloc + MMA issuer
+//   warps 2..9    rescale + epilogue: two warps per TMEM lane quarter, half the columns each
+#pragma once
+#include <cuda.h>
+
+#include "qlin_ptx.cuh"
+
+namespace qlin {
+
+struct Fp8Params {
+  int M, N;       // tokens, output channels
+  int kb;         // blocks of 128 along the contraction
+  int m_tiles, n_tiles;
+  const float* sx;  // [kb][ld_sx]
+  long long ld_sx;
+  const float* sw;  // block (output o, contraction r) at o * sw_out + r * sw_red
+  long long sw_out, sw_red;
+  const void* bias;
+  int bias_kind;    // 0 none, 1 f16, 2 f32, 3 bf16
+  void* y;
+  int y_dtype;      // OutDType
+  long long ldy;
+  int vec_out;      // rows of y take 16-byte stores
+  DeviceStatus* status;
+  // Element counts of the caller's buffers for the QLIN_CHECKS build (unused otherwise).
+  long long lim_y, lim_sx, lim_sw;
+};
+
+// Tokens by channels of one tile: CTAS = 2 is a cluster of two CTAs that share cta_group::2 MMAs of
+// 256 tokens x TN channels, each CTA holding its 128 tokens and half of the channels.
+template <int CTAS, int TN>
+struct Fp8Cfg {
+  static constexpr int kThreads = 320;
+  static constexpr int kBuf = 512 / TN;        // accumulator buffers in TMEM
+  static constexpr int kBRows = TN / CTAS;     // channels this CTA loads per stage
+  static constexpr uint32_t kAStage = 128 * 128;
+  static constexpr uint32_t kBStage = kBRows * 128;
+  static constexpr int kStages = 6;
+  static constexpr int kCols = TN / 2;         // accumulator columns per epilogue warp
+  static constexpr int kSmem = 1024 + kStages * (int)(kAStage + kBStage) + 512;
+  static_assert(CTAS == 1 || CTAS == 2, "one CTA or a pair");
+  static_assert(kBRows == 128, "the transposed operand is one 128-column block");
+};
+
+// Tiles in groups of kGroup token tiles, channels fastest within a group after the tokens: the tiles
+// that run at one time then share a few token tiles and a few channel tiles, which stay in L2.
+__device__ __forceinline__ void fp8_tile(int t, int m_tiles, int n_tiles, int& mt, int& nt) {
+  constexpr int kGroup = 8;
+  const int per = kGroup * n_tiles;
+  const int g = t / per, r = t - g * per;
+  const int rows = min(kGroup, m_tiles - g * kGroup);
+  nt = r / rows;
+  mt = g * kGroup + (r - nt * rows);
+}
+
+// (a0, a1) += s * (p0, p1)
+__device__ __forceinline__ void ffma2(float s, uint32_t p0, uint32_t p1, float& a0, float& a1) {
+  asm("{\n\t.reg .b64 f, sc, acc;\n\t"
+      "mov.b64 f, {%2, %3};\n\t"
+      "mov.b64 sc, {%4, %4};\n\t"
+      "mov.b64 acc, {%0, %1};\n\t"
+      "fma.rn.f32x2 acc, sc, f, acc;\n\t"
+      "mov.b64 {%0, %1}, acc;\n\t}"
+      : "+f"(a0), "+f"(a1)
+      : "r"(p0), "r"(p1), "f"(s));
+}
+
+__device__ __forceinline__ float fp8_bias(const void* bias, int kind, long long n, long long lim) {
+  if (kind == 0 || !qchk(BS_FP8_SCALE, n, lim)) return 0.f;
+  if (kind == 1) return __half2float(reinterpret_cast<const __half*>(bias)[n]);
+  if (kind == 2) return reinterpret_cast<const float*>(bias)[n];
+  return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(bias)[n]);
+}
+
+__device__ __forceinline__ uint32_t pack_out2(int dtype, float a, float b) {
+  if (dtype == OUT_F16) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <int CTAS, int TN, bool kTrans>
+__global__ void __launch_bounds__(320, 1)
+fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w,
+                const Fp8Params p) {
+  using Cfg = Fp8Cfg<CTAS, TN>;
+  constexpr int STAGES = Cfg::kStages;
+  constexpr int NB = Cfg::kBuf;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sa = smem;
+  uint8_t* sb = sa + STAGES * Cfg::kAStage;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sb + STAGES * Cfg::kBStage);
+  uint64_t* full = bars;              // [STAGES] both CTAs' operands landed (even CTA's)
+  uint64_t* empty = full + STAGES;    // [STAGES] MMAs that read the stage completed (each CTA's)
+  uint64_t* acc_full = empty + STAGES;   // [NB] products ready (each CTA's)
+  uint64_t* acc_empty = acc_full + NB;   // [NB] read out by the epilogue warps of both CTAs (even CTA's)
+  uint64_t* drain = acc_empty + NB;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = CTAS == 2 ? cluster_ctarank() : 0;
+  const int num_tiles = p.m_tiles * p.n_tiles;
+  const int tile0 = blockIdx.x / CTAS;
+  const int tile_step = gridDim.x / CTAS;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < NB; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 8 * CTAS);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    // the carve-out (rings, barriers, flags) lies inside the launch's shared memory
+    if (!qchk_smem(BS_FP8_SMEM, smem_raw, bars, reinterpret_cast<volatile uint8_t*>(abort_flag + 1) -
+                                          reinterpret_cast<volatile uint8_t*>(bars)))
+      *abort_flag = 1;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    if constexpr (CTAS == 2) {
+      tmem_alloc_pair(tmem_slot, 512);
+      tmem_relinquish_pair();
+    } else {
+      tmem_alloc(tmem_slot, 512);
+      tmem_relinquish();
+    }
+  }
+  if (warp == 0 && lane == 0 && p.kb > 0) {
+    prefetch_tmap(&tmap_x);
+    prefetch_tmap(&tmap_w);
+  }
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (CTAS == 2) cluster_sync();  // both CTAs' barriers are initialized before any remote arrive
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp == 0) {
+    // --------------------------------------------------------------------- producer (both CTAs)
+    if (elect_one()) {
+      const uint32_t full_leader = CTAS == 2 ? cluster_map(full, 0) : smem_u32(full);
+      uint32_t it = 0;
+      bool ok = true;
+      for (int t = tile0; t < num_tiles && ok; t += tile_step) {
+        int mt, nt;
+        fp8_tile(t, p.m_tiles, p.n_tiles, mt, nt);
+        const int m0 = (mt * CTAS + (int)rank) * 128;
+        const int n0 = nt * TN + (int)rank * Cfg::kBRows;
+        for (int b = 0; b < p.kb; ++b, ++it) {
+          const int s = it % STAGES;
+          if (!mbar_wait(&empty[s], ((it / STAGES) & 1) ^ 1, abort_flag, p.status, 0x41)) { ok = false; break; }
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], CTAS * (Cfg::kAStage + Cfg::kBStage));
+          const int wx = kTrans ? n0 : b * 128, wy = kTrans ? b * 128 : n0;
+          if constexpr (CTAS == 2) {
+            const uint32_t bar = full_leader + (uint32_t)(s * 8);
+            tma_load_2d_pair(sa + s * Cfg::kAStage, &tmap_x, bar, b * 128, m0);
+            tma_load_2d_pair(sb + s * Cfg::kBStage, &tmap_w, bar, wx, wy);
+          } else {
+            tma_load_2d(sa + s * Cfg::kAStage, &tmap_x, &full[s], b * 128, m0);
+            tma_load_2d(sb + s * Cfg::kBStage, &tmap_w, &full[s], wx, wy);
+          }
+        }
+      }
+      if (!ok && rank == 0) {  // wait for the copies in flight (the even CTA's barriers count both CTAs' bytes)
+        for (uint32_t j = (it >= (uint32_t)STAGES ? it - STAGES : 0); j < it; ++j) {
+          const uint64_t t0 = globaltimer();
+          while (!mbar_try_wait(smem_u32(&full[j % STAGES]), (j / STAGES) & 1)) {
+            if (globaltimer() - t0 > QLIN_WAIT_TIMEOUT_NS) break;
+          }
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // --------------------------------------------------------------------- MMA issuer (even CTA)
+    if (rank == 0 && elect_one()) {
+      constexpr uint32_t idesc = idesc_e4m3_f32(128 * CTAS, TN, false, kTrans);
+      // 32 contraction indices of one MMA: 32 bytes of a K-major row, or 32 rows of a transposed tile
+      constexpr uint64_t kBStep = kTrans ? (32 * 128) >> 4 : 32 >> 4;
+      uint32_t it = 0;
+      bool ok = true;
+      for (int t = tile0; t < num_tiles && ok; t += tile_step) {
+        for (int b = 0; b < p.kb; ++b, ++it) {
+          const int s = it % STAGES;
+          const uint32_t buf = it % NB;
+          if (!mbar_wait<CTAS == 2>(&full[s], (it / STAGES) & 1, abort_flag, p.status, 0x42) ||
+              !mbar_wait<CTAS == 2>(&acc_empty[buf], ((it / NB) & 1) ^ 1, abort_flag, p.status, 0x43)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t a_desc = smem_desc_sw128(smem_u32(sa + s * Cfg::kAStage));
+          const uint32_t sb_u = smem_u32(sb + s * Cfg::kBStage);
+          const uint64_t b_desc = kTrans ? smem_desc_sw128_mn(sb_u) : smem_desc_sw128(sb_u);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) {
+            const uint64_t ad = a_desc + (uint64_t)(kk * 2), bd = b_desc + (uint64_t)kk * kBStep;
+            if constexpr (CTAS == 2) mma_f8_ss_pair(tmem_base + buf * TN, ad, bd, idesc, kk > 0);
+            else mma_f8_ss(tmem_base + buf * TN, ad, bd, idesc, kk > 0);
+          }
+          if constexpr (CTAS == 2) {
+            tc_commit_pair(cluster_map(&acc_full[buf], 0));
+            tc_commit_pair(cluster_map(&acc_full[buf], 1));
+            tc_commit_pair(cluster_map(&empty[s], 0));
+            tc_commit_pair(cluster_map(&empty[s], 1));
+          } else {
+            tc_commit(&acc_full[buf]);
+            tc_commit(&empty[s]);
+          }
+        }
+      }
+      if constexpr (CTAS == 2) tc_commit_pair(cluster_map(drain, 0));
+      else tc_commit(drain);
+      const uint64_t t0 = globaltimer();
+      while (!mbar_try_wait(smem_u32(drain), 0)) {
+        if (globaltimer() - t0 > QLIN_WAIT_TIMEOUT_NS) break;
+      }
+    }
+  } else {
+    // --------------------------------------------------------------------- rescale + epilogue
+    constexpr int kCols = Cfg::kCols;
+    constexpr int kChunk = 16;
+    const int quarter = warp & 3;
+    const int part = (warp - 2) >> 2;
+    const int r = quarter * 32 + lane;  // TMEM lane == token within this CTA's 128
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const uint32_t acc_empty_leader = CTAS == 2 ? cluster_map(acc_empty, 0) : smem_u32(acc_empty);
+    uint32_t it = 0;
+    bool ok = true;
+    for (int t = tile0; t < num_tiles && ok; t += tile_step) {
+      int mt, nt;
+      fp8_tile(t, p.m_tiles, p.n_tiles, mt, nt);
+      const int m = (mt * CTAS + (int)rank) * 128 + r;
+      const int n0 = nt * TN + part * kCols;  // kCols channels from here, inside one 128-channel block
+      const bool m_ok = m < p.M;
+      const long long sw_off = (long long)min(n0 / 128, (p.N - 1) / 128) * p.sw_out;
+      float acc[kCols];
+#pragma unroll
+      for (int j = 0; j < kCols; ++j) acc[j] = 0.f;
+      auto load_sx = [&](int b) {
+        const long long i = (long long)b * p.ld_sx + m;
+        return (m_ok && b < p.kb && qchk(BS_FP8_SCALE, i, p.lim_sx)) ? __ldg(p.sx + i) : 0.f;
+      };
+      auto load_sw = [&](int b) {
+        const long long i = sw_off + (long long)b * p.sw_red;
+        return (b < p.kb && qchk(BS_FP8_SCALE, i, p.lim_sw)) ? __ldg(p.sw + i) : 0.f;
+      };
+      float sx = load_sx(0), sw = load_sw(0);  // the next block's scales are in flight during a block
+      for (int b = 0; b < p.kb; ++b, ++it) {
+        const float s = sx * sw;
+        sx = load_sx(b + 1);
+        sw = load_sw(b + 1);
+        const uint32_t buf = it % NB;
+        if (!mbar_wait(&acc_full[buf], (it / NB) & 1, abort_flag, p.status, 0x44)) { ok = false; break; }
+        tc_fence_after();
+        const uint32_t taddr = tmem_base + lanes + buf * TN + part * kCols;
+#pragma unroll
+        for (int c0 = 0; c0 < kCols; c0 += kChunk) {
+          uint32_t v[kChunk];
+          tmem_ld16(taddr + c0, v);
+          tmem_wait_ld();
+          if (c0 + kChunk >= kCols) {  // the last values are in registers: the buffer goes back to the issuer
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+              if constexpr (CTAS == 2) mbar_arrive_cluster(acc_empty_leader + buf * 8);
+              else mbar_arrive(&acc_empty[buf]);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < kChunk; j += 2) ffma2(s, v[j], v[j + 1], acc[c0 + j], acc[c0 + j + 1]);
+        }
+      }
+      if (!ok) break;
+      if (m_ok && n0 < p.N) {
+        const long long row = (long long)m * p.ldy;
+#pragma unroll
+        for (int c0 = 0; c0 < kCols; c0 += 8) {
+          const int n = n0 + c0;
+          float o[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) o[j] = acc[c0 + j] + (n + j < p.N ? fp8_bias(p.bias, p.bias_kind, n + j, p.N) : 0.f);
+          if (p.vec_out && n + 8 <= p.N && qchk_span(BS_FP8_Y, row + n, 8, p.lim_y)) {
+            if (p.y_dtype == OUT_F32) {
+              float4* y = reinterpret_cast<float4*>(reinterpret_cast<float*>(p.y) + row + n);
+              y[0] = make_float4(o[0], o[1], o[2], o[3]);
+              y[1] = make_float4(o[4], o[5], o[6], o[7]);
+            } else {
+              *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.y) + row + n) =
+                  make_uint4(pack_out2(p.y_dtype, o[0], o[1]), pack_out2(p.y_dtype, o[2], o[3]),
+                             pack_out2(p.y_dtype, o[4], o[5]), pack_out2(p.y_dtype, o[6], o[7]));
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              if (n + j >= p.N || !qchk(BS_FP8_Y, row + n + j, p.lim_y)) continue;
+              if (p.y_dtype == OUT_F32) reinterpret_cast<float*>(p.y)[row + n + j] = o[j];
+              else if (p.y_dtype == OUT_F16) reinterpret_cast<__half*>(p.y)[row + n + j] = __float2half_rn(o[j]);
+              else reinterpret_cast<__nv_bfloat16*>(p.y)[row + n + j] = __float2bfloat16_rn(o[j]);
+            }
+          }
+        }
+      }
+    }
+  }
+
+  // Warps 0 and 1 ran their loops on one elected lane; reconverge before the block barrier
+  // (barrier.sync is .aligned) and before the warp-wide TMEM dealloc.
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  // The even CTA's MMAs (which write the odd CTA's TMEM and read its shared memory) have all
+  // completed once its issuer's drain wait returned; neither CTA frees TMEM or exits before.
+  if constexpr (CTAS == 2) cluster_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    if constexpr (CTAS == 2) tmem_dealloc_pair(tmem_base, 512);
+    else tmem_dealloc(tmem_base, 512);
+  }
+}
+
+}  // namespace qlin

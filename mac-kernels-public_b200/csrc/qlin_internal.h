@@ -122,5 +122,7 @@ int bounds_read_f16_blk(BoundsRecord* out, int reset);
 int bounds_read_f16_kq(BoundsRecord* out, int reset);
 int bounds_read_gemv(BoundsRecord* out, int reset);
 int bounds_read_i8(BoundsRecord* out, int reset);
+int bounds_read_fp8(BoundsRecord* out, int reset);
+int bounds_read_rotary(BoundsRecord* out, int reset);
 
 }  // namespace qlin

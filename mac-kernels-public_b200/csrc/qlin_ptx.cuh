@@ -166,6 +166,17 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const void* tmap, uint64_
       : "memory");
 }
 
+// The same load by either CTA of a pair into its own shared memory, its bytes counted on a barrier of
+// either CTA (a shared::cluster address, e.g. the even CTA's).
+__device__ __forceinline__ void tma_load_2d_pair(void* dst, const void* tmap, uint32_t bar_cluster, int32_t x,
+                                                 int32_t y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], "
+      "[%2];" ::"r"(smem_u32(dst)),
+      "l"(tmap), "r"(bar_cluster), "r"(x), "r"(y)
+      : "memory");
+}
+
 __device__ __forceinline__ void tma_load_3d(void* dst, const void* tmap, uint64_t* bar, int32_t x, int32_t y,
                                             int32_t z) {
   asm volatile(
@@ -306,6 +317,26 @@ __device__ __forceinline__ void mma_f16_ts_pair(uint32_t d_tmem, uint32_t a_tmem
       "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
+// D[tmem] (+)= A[smem desc] * B[smem desc]^T, kind::f8f6f4 (8-bit floats, fp32 accumulate).
+__device__ __forceinline__ void mma_f8_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                          uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// The pair form: A is 128 rows of each CTA's shared memory, B and D as for mma_f16_ts_pair.
+__device__ __forceinline__ void mma_f8_ss_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                               uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
 // Arrive on the mbarrier at a shared::cluster address (either CTA of the pair) once every
 // previously issued pair MMA of this thread completed.
 __device__ __forceinline__ void tc_commit_pair(uint32_t cluster_addr) {
@@ -411,6 +442,19 @@ __device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t smem_addr) {
   return d;
 }
 
+// The same for a transposed 128-column operand: rows of 128 bytes are contraction indices, so the
+// 8-row groups 1024 bytes apart step along K (32 indices of one kind::f8f6f4 MMA: four groups) and
+// the stride between 128-column blocks is not used.
+__device__ __forceinline__ uint64_t smem_desc_sw128_mn(uint32_t smem_addr) {
+  uint64_t d = 0;
+  d |= (uint64_t)((smem_addr & 0x3FFFF) >> 4);
+  d |= (uint64_t)(1024 >> 4) << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+
 // Instruction descriptor, dense, both operands K-major.
 //   c_format [4,6): 1 = f32, 2 = s32;  a/b format [7,10)/[10,13): f16 = 0, bf16 = 1 (kind::f16), s8 = 1 (kind::i8)
 //   n_dim [17,23) = N >> 3;  m_dim [24,29) = M >> 4
@@ -419,6 +463,12 @@ __host__ __device__ constexpr uint32_t idesc_f16_f32(uint32_t m, uint32_t n) {
 }
 __host__ __device__ constexpr uint32_t idesc_bf16_f32(uint32_t m, uint32_t n) {
   return (1u << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+// e4m3 x e4m3 -> f32 (kind::f8f6f4).  Transposed A (bit 15) / B (bit 16): that operand's tile lies with
+// its M / N index contiguous, 128 of them to a swizzled 128-byte row, one row per contraction index.
+__host__ __device__ constexpr uint32_t idesc_e4m3_f32(uint32_t m, uint32_t n, bool trans_a, bool trans_b) {
+  return (1u << 4) | (0u << 7) | (0u << 10) | ((trans_a ? 1u : 0u) << 15) | ((trans_b ? 1u : 0u) << 16) |
+         ((n >> 3) << 17) | ((m >> 4) << 24);
 }
 __host__ __device__ constexpr uint32_t idesc_s8_s32(uint32_t m, uint32_t n) {
   return (2u << 4) | (1u << 7) | (1u << 10) | ((n >> 3) << 17) | ((m >> 4) << 24);

@@ -1,0 +1,839 @@
+// Rotary positions with several axes, and the RMS norm of every query and key head with the position
+// rotation in the same pass, forward and backward.
+//
+// Table: pair p of a head belongs to one axis a and turns by angle = pos[a] * theta^(-2 i / dim_a), i its
+// index within the axis; the table holds (cos, sin) in fp32, [tokens][pairs][2].
+//
+// Head norm with rotation, for each head's row x of D values with weight w:
+//   v = x * rstd * w,  rstd = (mean(x^2) + eps)^-1/2
+//   (y_a, y_b) = (v_a c - v_b s, v_a s + v_b c) for each rotated pair; the values past 2 * pairs stay v
+// A pair is two neighbours (interleaved) or the same place of the rotated part's two halves.
+// Backward, with g the gradient rotated back and xhat = x * rstd:
+//   dx = rstd * (g w - xhat * mean(g w xhat)),  dw = sum over all rows of g * xhat
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "../../include/qlin.h"
+#include "qlin_internal.h"
+#include "qlin_ptx.cuh"
+
+namespace qlin {
+
+// ---------------------------------------------------------------------------------------------
+// Table
+// ---------------------------------------------------------------------------------------------
+constexpr int kMaxPairs = 256;
+
+struct RotTableParams {
+  const void* pos;  // [tokens, axes]
+  long long tokens;
+  int axes, pairs;
+  float2* out;      // [tokens, pairs]
+  double turns[kMaxPairs];         // theta^(-2 i / dim) / (2 pi) of each pair
+  unsigned char axis[kMaxPairs];
+};
+
+__device__ __forceinline__ double load_pos(const void* p, int kind, long long i) {
+  if (kind == QLIN_F32) return (double)reinterpret_cast<const float*>(p)[i];
+  if (kind == QLIN_I32) return (double)reinterpret_cast<const int*>(p)[i];
+  return (double)reinterpret_cast<const long long*>(p)[i];
+}
+
+// The angle is kept in turns and in 64 bits until its whole turns are gone, so large positions lose
+// nothing; what is left, at most half a turn, is exact to fp32 rounding for sincospif.  A thread keeps its
+// pair's frequency and walks over tokens, a warp writes 256 consecutive bytes.
+template <int KIND>
+__global__ void __launch_bounds__(256) rotary_table_kernel(const __grid_constant__ RotTableParams p) {
+  const int pair = blockIdx.y * 32 + threadIdx.x;
+  if (pair >= p.pairs) return;
+  const double turns = p.turns[pair];
+  const int axis = p.axis[pair];
+  for (long long t = (long long)blockIdx.x * 8 + threadIdx.y; t < p.tokens; t += (long long)gridDim.x * 8) {
+    if (!qchk(BS_ROT_IN, t * p.axes + axis, p.tokens * p.axes) ||
+        !qchk(BS_ROT_OUT, t * p.pairs + pair, p.tokens * p.pairs))
+      continue;
+    double u = load_pos(p.pos, KIND, t * p.axes + axis) * turns;
+    u -= rint(u);
+    float s, c;
+    sincospif(2.f * (float)u, &s, &c);
+    p.out[t * p.pairs + pair] = make_float2(c, s);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Head norm with rotation
+// ---------------------------------------------------------------------------------------------
+// One of q and k: [B, L, heads, D] with element strides, values of a row side by side.
+struct HeadSide {
+  const void* x;
+  const void* dy;      // backward: the output's gradient
+  void* y;             // forward: the output; backward: dx
+  const void* w;       // [D] or null
+  float* dw;           // backward: partial sums [ctas][D]
+  int heads, chunks;   // chunks: warps that share a token's heads
+  long long x_b, x_l, x_h, y_b, y_l, y_h, dy_b, dy_l, dy_h;
+  long long lim_x, lim_y, lim_dy;  // element counts for the QLIN_CHECKS build
+};
+
+struct HeadParams {
+  HeadSide side[2];    // q, k
+  const float2* table;
+  long long table_b;   // float2 between batches (0: shared)
+  long long tokens;    // B * L
+  int L, D, pairs;     // pairs: rotated pairs of a head
+  int interleaved;
+  float eps;
+  int w_dtype;
+  int heads_per_warp;
+  int ctas[2];         // backward: CTAs of each side
+  long long lim_table;
+};
+
+template <int DT>
+__device__ __forceinline__ float head_load(const void* x, long long i) {
+  if constexpr (DT == QLIN_F16) return __half2float(reinterpret_cast<const __half*>(x)[i]);
+  else if constexpr (DT == QLIN_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(x)[i]);
+  else return reinterpret_cast<const float*>(x)[i];
+}
+template <int DT>
+__device__ __forceinline__ void head_store(void* x, long long i, float v) {
+  if constexpr (DT == QLIN_F16) reinterpret_cast<__half*>(x)[i] = __float2half_rn(v);
+  else if constexpr (DT == QLIN_BF16) reinterpret_cast<__nv_bfloat16*>(x)[i] = __float2bfloat16_rn(v);
+  else reinterpret_cast<float*>(x)[i] = v;
+}
+__device__ __forceinline__ float weight_at(const void* w, int dt, int i, int D) {
+  if (w == nullptr || !qchk(BS_ROT_IN, i, D)) return 1.f;
+  if (dt == QLIN_F16) return __half2float(reinterpret_cast<const __half*>(w)[i]);
+  if (dt == QLIN_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(w)[i]);
+  return reinterpret_cast<const float*>(w)[i];
+}
+
+// A lane's 8 values of a row: two pieces of 4, at o0 and o1.  Interleaved (and past the rotated part) the
+// pieces are neighbours and hold pairs (0,1) (2,3) | (4,5) (6,7); with halves, pair i is value i of each piece.
+template <int DT>
+struct Pieces {
+  uint2 v[DT == QLIN_F32 ? 4 : 2];
+};
+
+template <int DT, bool kInter>
+__device__ __forceinline__ Pieces<DT> load_pieces(const void* x, long long row, int o0, int o1) {
+  Pieces<DT> r;
+  if constexpr (DT == QLIN_F32) {
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(x) + row + o0));
+    const uint4 b = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(x) + row + o1));
+    r.v[0] = make_uint2(a.x, a.y);
+    r.v[1] = make_uint2(a.z, a.w);
+    r.v[2] = make_uint2(b.x, b.y);
+    r.v[3] = make_uint2(b.z, b.w);
+  } else if constexpr (kInter) {
+    const uint4 a = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(x) + row + o0));
+    r.v[0] = make_uint2(a.x, a.y);
+    r.v[1] = make_uint2(a.z, a.w);
+  } else {
+    r.v[0] = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(x) + row + o0));
+    r.v[1] = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(x) + row + o1));
+  }
+  return r;
+}
+
+template <int DT>
+__device__ __forceinline__ void pieces_to_float(const Pieces<DT>& r, float (&f)[8]) {
+#pragma unroll
+  for (int i = 0; i < (DT == QLIN_F32 ? 4 : 2); ++i) {
+    const uint32_t w[2] = {r.v[i].x, r.v[i].y};
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if constexpr (DT == QLIN_F32) {
+        f[2 * i + j] = __uint_as_float(w[j]);
+      } else if constexpr (DT == QLIN_F16) {
+        const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+        f[4 * i + 2 * j] = t.x;
+        f[4 * i + 2 * j + 1] = t.y;
+      } else {
+        f[4 * i + 2 * j] = __uint_as_float(w[j] << 16);
+        f[4 * i + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+      }
+    }
+  }
+}
+
+template <int DT, bool kInter>
+__device__ __forceinline__ void store_pieces(void* y, long long row, int o0, int o1, const float (&f)[8]) {
+  if constexpr (DT == QLIN_F32) {
+    float* p = reinterpret_cast<float*>(y) + row;
+    *reinterpret_cast<float4*>(p + o0) = make_float4(f[0], f[1], f[2], f[3]);
+    *reinterpret_cast<float4*>(p + o1) = make_float4(f[4], f[5], f[6], f[7]);
+  } else {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (DT == QLIN_F16) {
+        const __half2 h = __floats2half2_rn(f[2 * j], f[2 * j + 1]);
+        w[j] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(f[2 * j], f[2 * j + 1]);
+        w[j] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+    uint16_t* p = reinterpret_cast<uint16_t*>(y) + row;
+    if constexpr (kInter) {
+      *reinterpret_cast<uint4*>(p + o0) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+      *reinterpret_cast<uint2*>(p + o0) = make_uint2(w[0], w[1]);
+      *reinterpret_cast<uint2*>(p + o1) = make_uint2(w[2], w[3]);
+    }
+  }
+}
+
+// Rotates the lane's 4 pairs in place by (c, s); kBack by (c, -s).
+template <bool kInter, bool kBack>
+__device__ __forceinline__ void rotate4(float (&f)[8], const float (&c)[4], const float (&s)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int a = kInter ? 2 * i : i, b = kInter ? 2 * i + 1 : i + 4;
+    const float sn = kBack ? -s[i] : s[i];
+    const float t = f[a] * c[i] - f[b] * sn;
+    f[b] = f[a] * sn + f[b] * c[i];
+    f[a] = t;
+  }
+}
+
+// What a lane does in every row: where its values lie, and its pairs' place in the table (-1: not rotated).
+template <int G>
+struct LanePlan {
+  int o0, o1, pair0;
+  bool on;
+  __device__ __forceinline__ LanePlan(int lane, int D, int pairs, bool inter) {
+    const int j = lane & (G - 1);
+    on = j * 8 < D;
+    o0 = j * 8;
+    o1 = o0 + 4;
+    pair0 = -1;
+    if (j * 4 < pairs) {
+      pair0 = j * 4;
+      if (!inter) {
+        o0 = j * 4;
+        o1 = o0 + pairs;
+      }
+    }
+  }
+};
+
+__device__ __forceinline__ void load_turn(const HeadParams& p, long long token_row, int pair0, float (&c)[4],
+                                          float (&s)[4]) {
+  if (pair0 >= 0 && qchk_span(BS_ROT_IN, token_row + pair0, 4, p.lim_table)) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(p.table + token_row + pair0));
+    const float4 b = __ldg(reinterpret_cast<const float4*>(p.table + token_row + pair0) + 1);
+    c[0] = a.x; s[0] = a.y; c[1] = a.z; s[1] = a.w;
+    c[2] = b.x; s[2] = b.y; c[3] = b.z; s[3] = b.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      c[i] = 1.f;
+      s[i] = 0.f;
+    }
+  }
+}
+
+template <int G>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+  for (int o = G / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// Forward.  A row is G lanes of 8 values; a warp takes one token's q or k heads (or a share of them, where
+// there are few tokens), 32 / G rows at a time with kUnroll loads in flight, and keeps the token's cosines
+// and sines and the weight in registers.
+template <int DT, int G, bool kInter>
+__global__ void __launch_bounds__(256) qk_norm_rotary_kernel(const __grid_constant__ HeadParams p) {
+  constexpr int R = 32 / G;
+  constexpr int kUnroll = 4;
+  const int lane = threadIdx.x & 31;
+  const long long item = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int per = p.side[0].chunks + p.side[1].chunks;
+  const long long token = item / per;
+  if (token >= p.tokens) return;
+  int chunk = (int)(item - token * per);
+  const int which = chunk >= p.side[0].chunks ? 1 : 0;
+  if (which) chunk -= p.side[0].chunks;
+  const HeadSide& sd = p.side[which];
+  const long long b = token / p.L, l = token - b * p.L;
+  const LanePlan<G> plan(lane, p.D, p.pairs, kInter);
+  float c[4], s[4], w[8];
+  load_turn(p, b * p.table_b + l * p.pairs, plan.pair0, c, s);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) w[j] = plan.on ? weight_at(sd.w, p.w_dtype, (j < 4 ? plan.o0 : plan.o1 - 4) + j, p.D) : 0.f;
+  const float inv_d = 1.f / (float)p.D;
+  const long long xr = b * sd.x_b + l * sd.x_l, yr = b * sd.y_b + l * sd.y_l;
+  const int h_end = min(sd.heads, (chunk + 1) * p.heads_per_warp);
+  for (int h0 = chunk * p.heads_per_warp; h0 < h_end; h0 += R * kUnroll) {
+    Pieces<DT> raw[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int h = h0 + u * R + lane / G;
+      raw[u] = Pieces<DT>{};
+      const long long row = xr + (long long)h * sd.x_h;
+      if (h < h_end && plan.on && qchk_span(BS_ROT_IN, row + plan.o0, 4, sd.lim_x) &&
+          qchk_span(BS_ROT_IN, row + plan.o1, 4, sd.lim_x))
+        raw[u] = load_pieces<DT, kInter>(sd.x, row, plan.o0, plan.o1);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int h = h0 + u * R + lane / G;
+      float f[8], ss = 0.f;
+      pieces_to_float<DT>(raw[u], f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) ss = fmaf(f[j], f[j], ss);
+      const float rstd = rsqrtf(group_sum<G>(ss) * inv_d + p.eps);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = f[j] * rstd * w[j];
+      rotate4<kInter, false>(f, c, s);
+      const long long row = yr + (long long)h * sd.y_h;
+      if (h < h_end && plan.on && qchk_span(BS_ROT_OUT, row + plan.o0, 4, sd.lim_y) &&
+          qchk_span(BS_ROT_OUT, row + plan.o1, 4, sd.lim_y))
+        store_pieces<DT, kInter>(sd.y, row, plan.o0, plan.o1, f);
+    }
+  }
+}
+
+// Backward.  The CTAs of a side walk over its (token, share of heads) items; every lane sums its 8 columns'
+// g * xhat in fp32, the CTA joins its rows in a fixed order and leaves one partial row of dw, and the
+// kernel below adds those up, also in a fixed order.
+template <int DT, int G, bool kInter>
+__global__ void __launch_bounds__(256) qk_norm_rotary_bwd_kernel(const __grid_constant__ HeadParams p) {
+  constexpr int R = 32 / G;
+  constexpr int kUnroll = 2;
+  __shared__ float part[8 * R][G * 8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int which = blockIdx.x >= (unsigned)p.ctas[0] ? 1 : 0;
+  const int cta = which ? blockIdx.x - p.ctas[0] : blockIdx.x;
+  const HeadSide& sd = p.side[which];
+  const LanePlan<G> plan(lane, p.D, p.pairs, kInter);
+  float w[8], dw[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    w[j] = plan.on ? weight_at(sd.w, p.w_dtype, (j < 4 ? plan.o0 : plan.o1 - 4) + j, p.D) : 0.f;
+    dw[j] = 0.f;
+  }
+  const float inv_d = 1.f / (float)p.D;
+  const long long items = p.tokens * sd.chunks;
+  for (long long item = (long long)cta * 8 + warp; item < items; item += (long long)p.ctas[which] * 8) {
+    const long long token = item / sd.chunks;
+    const int chunk = (int)(item - token * sd.chunks);
+    const long long b = token / p.L, l = token - b * p.L;
+    float c[4], s[4];
+    load_turn(p, b * p.table_b + l * p.pairs, plan.pair0, c, s);
+    const long long xr = b * sd.x_b + l * sd.x_l, yr = b * sd.y_b + l * sd.y_l, gr = b * sd.dy_b + l * sd.dy_l;
+    const int h_end = min(sd.heads, (chunk + 1) * p.heads_per_warp);
+    for (int h0 = chunk * p.heads_per_warp; h0 < h_end; h0 += R * kUnroll) {
+      Pieces<DT> rx[kUnroll], rg[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int h = h0 + u * R + lane / G;
+        rx[u] = Pieces<DT>{};
+        rg[u] = Pieces<DT>{};
+        const long long row = xr + (long long)h * sd.x_h, grow = gr + (long long)h * sd.dy_h;
+        if (h < h_end && plan.on && qchk_span(BS_ROT_IN, row + plan.o0, 4, sd.lim_x) &&
+            qchk_span(BS_ROT_IN, row + plan.o1, 4, sd.lim_x) &&
+            qchk_span(BS_ROT_IN, grow + plan.o0, 4, sd.lim_dy) && qchk_span(BS_ROT_IN, grow + plan.o1, 4, sd.lim_dy)) {
+          rx[u] = load_pieces<DT, kInter>(sd.x, row, plan.o0, plan.o1);
+          rg[u] = load_pieces<DT, kInter>(sd.dy, grow, plan.o0, plan.o1);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int h = h0 + u * R + lane / G;
+        float x[8], g[8], ss = 0.f, dot = 0.f;
+        pieces_to_float<DT>(rx[u], x);
+        pieces_to_float<DT>(rg[u], g);
+        rotate4<kInter, true>(g, c, s);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          ss = fmaf(x[j], x[j], ss);
+          dot = fmaf(g[j] * w[j], x[j], dot);
+        }
+        ss = group_sum<G>(ss);
+        dot = group_sum<G>(dot);
+        const float rstd = rsqrtf(ss * inv_d + p.eps);
+        const float pull = rstd * rstd * (dot * inv_d);
+        if (h < h_end) {
+          float o[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            dw[j] = fmaf(g[j], x[j] * rstd, dw[j]);
+            o[j] = rstd * (g[j] * w[j] - x[j] * pull);
+          }
+          const long long row = yr + (long long)h * sd.y_h;
+          if (plan.on && qchk_span(BS_ROT_OUT, row + plan.o0, 4, sd.lim_y) &&
+              qchk_span(BS_ROT_OUT, row + plan.o1, 4, sd.lim_y))
+            store_pieces<DT, kInter>(sd.y, row, plan.o0, plan.o1, o);
+        }
+      }
+    }
+  }
+  if (sd.dw == nullptr) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (plan.on) part[warp * R + lane / G][(j < 4 ? plan.o0 : plan.o1 - 4) + j] = dw[j];
+  __syncthreads();
+  for (int i = threadIdx.x; i < p.D; i += 256) {
+    float sum = 0.f;
+#pragma unroll
+    for (int r = 0; r < 8 * R; ++r) sum += part[r][i];
+    const long long at = (long long)cta * p.D + i;
+    if (qchk(BS_ROT_OUT, at, (long long)p.ctas[which] * p.D)) sd.dw[at] = sum;
+  }
+}
+
+struct DwParams {
+  const float* part[2];
+  int ctas[2];
+  void* out[2];
+  int D, w_dtype;
+};
+
+// dw = the sum of the partial rows: 32 columns to a CTA, 32 rows at a time, one rounding to the weight's type.
+__global__ void __launch_bounds__(1024) dw_sum_kernel(const DwParams p) {
+  __shared__ float part[32][33];
+  const int which = blockIdx.y;
+  const int i = blockIdx.x * 32 + threadIdx.x;
+  if (p.out[which] == nullptr) return;
+  float sum = 0.f;
+  if (i < p.D)
+    for (int r = threadIdx.y; r < p.ctas[which]; r += 32)
+      if (qchk(BS_ROT_IN, (long long)r * p.D + i, (long long)p.ctas[which] * p.D))
+        sum += p.part[which][(long long)r * p.D + i];
+  part[threadIdx.y][threadIdx.x] = sum;
+  __syncthreads();
+  float v = part[threadIdx.x][threadIdx.y];  // warp y: the 32 partial sums of column y
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  const int col = blockIdx.x * 32 + threadIdx.y;
+  if (threadIdx.x == 0 && col < p.D && qchk(BS_ROT_OUT, col, p.D)) {
+    if (p.w_dtype == QLIN_F16) head_store<QLIN_F16>(p.out[which], col, v);
+    else if (p.w_dtype == QLIN_BF16) head_store<QLIN_BF16>(p.out[which], col, v);
+    else head_store<QLIN_F32>(p.out[which], col, v);
+  }
+}
+
+// Any head size and alignment: one warp to a row, values one by one, the row read twice (the second time
+// from the cache).  kBack: the gradients; dw goes to one partial row per CTA as above, summed by each CTA over
+// its own rows in shared memory (D <= 1024), every column always by the same thread's warp in row order.
+template <int DT, bool kBack>
+__global__ void __launch_bounds__(256) qk_norm_rotary_any_kernel(const __grid_constant__ HeadParams p) {
+  extern __shared__ float warp_dw[];  // backward: [8][D]
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int which = blockIdx.x >= (unsigned)p.ctas[0] ? 1 : 0;
+  const int cta = which ? blockIdx.x - p.ctas[0] : blockIdx.x;
+  const HeadSide& sd = p.side[which];
+  if constexpr (kBack)
+    for (int i = lane; i < p.D; i += 32) warp_dw[warp * p.D + i] = 0.f;
+  __syncwarp();
+  const float inv_d = 1.f / (float)p.D;
+  const long long rows = p.tokens * sd.heads;
+  const int rot = 2 * p.pairs;
+  for (long long row = (long long)cta * 8 + warp; row < rows; row += (long long)p.ctas[which] * 8) {
+    const long long token = row / sd.heads, h = row - token * sd.heads;
+    const long long b = token / p.L, l = token - b * p.L;
+    const long long xr = b * sd.x_b + l * sd.x_l + h * sd.x_h, yr = b * sd.y_b + l * sd.y_l + h * sd.y_h;
+    const long long gr = b * sd.dy_b + l * sd.dy_l + h * sd.dy_h;
+    const long long tr = b * p.table_b + l * p.pairs;
+    auto x_at = [&](int i) { return qchk(BS_ROT_IN, xr + i, sd.lim_x) ? head_load<DT>(sd.x, xr + i) : 0.f; };
+    auto dy_at = [&](int i) { return qchk(BS_ROT_IN, gr + i, sd.lim_dy) ? head_load<DT>(sd.dy, gr + i) : 0.f; };
+    auto put = [&](int i, float v) {
+      if (qchk(BS_ROT_OUT, yr + i, sd.lim_y)) head_store<DT>(sd.y, yr + i, v);
+    };
+    // item i < pairs: a rotated pair; past that: one plain value
+    const int items = p.pairs + (p.D - rot);
+    auto place = [&](int i, int& a, int& bb) {
+      if (i >= p.pairs) a = bb = rot + (i - p.pairs);
+      else if (p.interleaved) { a = 2 * i; bb = a + 1; }
+      else { a = i; bb = i + p.pairs; }
+    };
+    auto grads = [&](int i, int a, int bb, float& ga, float& gb) {  // the gradient, rotated back
+      ga = dy_at(a);
+      gb = a == bb ? 0.f : dy_at(bb);
+      if (i < p.pairs && qchk(BS_ROT_IN, tr + i, p.lim_table)) {
+        const float2 t = __ldg(p.table + tr + i);
+        const float v = ga * t.x + gb * t.y;
+        gb = gb * t.x - ga * t.y;
+        ga = v;
+      }
+    };
+    float ss = 0.f, dot = 0.f;
+    for (int i = lane; i < items; i += 32) {
+      int a, bb;
+      place(i, a, bb);
+      const float xa = x_at(a), xb = a == bb ? 0.f : x_at(bb);
+      ss += xa * xa + xb * xb;
+      if constexpr (kBack) {
+        float ga, gb;
+        grads(i, a, bb, ga, gb);
+        dot += ga * weight_at(sd.w, p.w_dtype, a, p.D) * xa + gb * weight_at(sd.w, p.w_dtype, bb, p.D) * xb;
+      }
+    }
+    const float rstd = rsqrtf(group_sum<32>(ss) * inv_d + p.eps);
+    if constexpr (kBack) dot = group_sum<32>(dot);
+    for (int i = lane; i < items; i += 32) {
+      int a, bb;
+      place(i, a, bb);
+      const float xa = x_at(a), xb = a == bb ? 0.f : x_at(bb);
+      const float wa = weight_at(sd.w, p.w_dtype, a, p.D), wb = weight_at(sd.w, p.w_dtype, bb, p.D);
+      if constexpr (kBack) {
+        float ga, gb;
+        grads(i, a, bb, ga, gb);
+        const float pull = rstd * rstd * (dot * inv_d);
+        warp_dw[warp * p.D + a] += ga * (xa * rstd);
+        if (a != bb) warp_dw[warp * p.D + bb] += gb * (xb * rstd);
+        put(a, rstd * (ga * wa - xa * pull));
+        if (a != bb) put(bb, rstd * (gb * wb - xb * pull));
+      } else {
+        const float va = xa * rstd * wa, vb = xb * rstd * wb;
+        float2 t = make_float2(1.f, 0.f);
+        if (i < p.pairs && qchk(BS_ROT_IN, tr + i, p.lim_table)) t = __ldg(p.table + tr + i);
+        put(a, va * t.x - vb * t.y);
+        if (a != bb) put(bb, va * t.y + vb * t.x);
+      }
+    }
+  }
+  if constexpr (kBack) {
+    if (sd.dw == nullptr) return;
+    __syncthreads();
+    for (int i = threadIdx.x; i < p.D; i += 256) {
+      float sum = 0.f;
+      for (int r = 0; r < 8; ++r) sum += warp_dw[r * p.D + i];
+      const long long at = (long long)cta * p.D + i;
+      if (qchk(BS_ROT_OUT, at, (long long)p.ctas[which] * p.D)) sd.dw[at] = sum;
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------------------------
+static int rot_launched(const char* what) {
+  const cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) return QLIN_OK;
+  set_error("%s: %s", what, cudaGetErrorString(e));
+  return QLIN_ECUDA;
+}
+
+constexpr int kMaxHeadDim = 1024;
+
+// The vector kernels take heads of whole 8-value pieces up to 256, rotated parts of whole pieces, and rows
+// that start on the pieces' alignment.
+static bool head_rows_aligned(const void* p, long long sb, long long sl, long long sh, int dtype, bool inter) {
+  const int esz = dtype == QLIN_F32 ? 4 : 2;
+  const uintptr_t al = dtype == QLIN_F32 || inter ? 16 : 8;
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(p) | (uintptr_t)(sb * esz) | (uintptr_t)(sl * esz) |
+                         (uintptr_t)(sh * esz);
+  return bits % al == 0;
+}
+
+static int lanes_per_row(int D) {
+  int g = 4;
+  while (g * 8 < D) g *= 2;
+  return g;
+}
+
+// Backward: the CTAs of both sides together, each with a partial row of dw.  Four resident CTAs on each SM
+// or fewer where there are fewer rows.
+static void plan_bwd(long long tokens, int hq, int hk, int rows_per_cta, int (&ctas)[2]) {
+  const long long most = 4ll * sm_count();
+  const long long rows = tokens * (hq + hk);
+  const long long want = std::max<long long>(2, std::min<long long>(most, rows / rows_per_cta));
+  const int heads[2] = {hq, hk};
+  for (int i = 0; i < 2; ++i)
+    ctas[i] = heads[i] == 0 ? 0 : (int)std::max<long long>(1, want * heads[i] / (hq + hk));
+}
+
+template <int DT, bool kInter>
+static void launch_rows(const HeadParams& p, int g, bool back, unsigned grid, cudaStream_t s) {
+  switch (g) {
+#define QLIN_ROWS(G)                                                                    \
+  case G:                                                                               \
+    if (back) qk_norm_rotary_bwd_kernel<DT, G, kInter><<<grid, 256, 0, s>>>(p);         \
+    else qk_norm_rotary_kernel<DT, G, kInter><<<grid, 256, 0, s>>>(p);                  \
+    break;
+    QLIN_ROWS(4)
+    QLIN_ROWS(8)
+    QLIN_ROWS(16)
+    QLIN_ROWS(32)
+#undef QLIN_ROWS
+  }
+}
+
+template <int DT>
+static void launch_dtype(const HeadParams& p, bool vec, bool back, unsigned grid, cudaStream_t s) {
+  if (!vec) {
+    if (back) qk_norm_rotary_any_kernel<DT, true><<<grid, 256, (size_t)8 * p.D * 4, s>>>(p);
+    else qk_norm_rotary_any_kernel<DT, false><<<grid, 256, 0, s>>>(p);
+  } else if (p.interleaved) {
+    launch_rows<DT, true>(p, lanes_per_row(p.D), back, grid, s);
+  } else {
+    launch_rows<DT, false>(p, lanes_per_row(p.D), back, grid, s);
+  }
+}
+
+static long long reach(long long n0, long long s0, long long n1, long long s1, long long n2, long long s2, long long d) {
+  return (n0 - 1) * s0 + (n1 - 1) * s1 + (n2 - 1) * s2 + d;
+}
+
+// Rows a backward CTA should have at least: each of its partial rows costs D values of traffic again.
+constexpr int kBwdRowsPerCta = 64;
+
+static size_t bwd_workspace(long long tokens, int hq, int hk, int D) {
+  int ctas[2];
+  plan_bwd(tokens, hq, hk, kBwdRowsPerCta, ctas);
+  return (size_t)(ctas[0] + ctas[1]) * D * 4;
+}
+
+struct HeadCall {
+  const char* what;
+  bool back;
+  const void *q, *k, *dq, *dk;
+  void *oq, *ok;
+  const int64_t *q_strides, *k_strides, *dq_strides, *dk_strides, *oq_strides, *ok_strides;
+  void *dqw, *dkw;
+};
+
+static int head_norm(const HeadCall& a, int dtype, int64_t batch, int64_t tokens, int hq, int hk, int dim, const void* qw,
+                     const void* kw, int w_dtype, const float* table, int64_t table_batch_stride, int pairs,
+                     float eps, int interleaved, void* workspace, size_t workspace_bytes, cudaStream_t stream) {
+  if (batch < 0 || tokens < 0 || hq < 0 || hk < 0 || dim <= 0 || pairs < 0 || 2 * pairs > dim ||
+      tokens > 0x7fffffff || (table_batch_stride != 0 && table_batch_stride < tokens * pairs * 2)) {
+    set_error("%s: bad sizes batch=%lld tokens=%lld heads=%d,%d dim=%d pairs=%d", a.what, (long long)batch,
+              (long long)tokens, hq, hk, dim, pairs);
+    return QLIN_EINVAL;
+  }
+  const bool floats = (dtype == QLIN_F32 || dtype == QLIN_F16 || dtype == QLIN_BF16) &&
+                      (w_dtype == QLIN_F32 || w_dtype == QLIN_F16 || w_dtype == QLIN_BF16);
+  if (!floats || dim > kMaxHeadDim || table_batch_stride % 2 != 0 || (reinterpret_cast<uintptr_t>(table) & 7)) {
+    set_error("%s: heads of up to %d values in f32, f16 or bf16, an 8-byte aligned table", a.what, kMaxHeadDim);
+    return QLIN_EDECLINE;
+  }
+  const int64_t rows = batch * tokens;
+  if (rows == 0 || hq + hk == 0) {
+    const int wsz = w_dtype == QLIN_F32 ? 4 : 2;  // no rows: the weights' gradients are zeros
+    if (a.dqw != nullptr && cudaMemsetAsync(a.dqw, 0, (size_t)dim * wsz, stream) != cudaSuccess) return rot_launched(a.what);
+    if (a.dkw != nullptr && cudaMemsetAsync(a.dkw, 0, (size_t)dim * wsz, stream) != cudaSuccess) return rot_launched(a.what);
+    return QLIN_OK;
+  }
+  if ((hq > 0 && (a.q == nullptr || a.oq == nullptr || (a.back && a.dq == nullptr))) ||
+      (hk > 0 && (a.k == nullptr || a.ok == nullptr || (a.back && a.dk == nullptr))) || (pairs > 0 && table == nullptr)) {
+    set_error("%s: null pointer", a.what);
+    return QLIN_EINVAL;
+  }
+  HeadParams p{};
+  p.table = reinterpret_cast<const float2*>(table);
+  p.table_b = table_batch_stride / 2;
+  p.tokens = rows;
+  p.L = (int)tokens;
+  p.D = dim;
+  p.pairs = pairs;
+  p.interleaved = interleaved ? 1 : 0;
+  p.eps = eps;
+  p.w_dtype = w_dtype;
+  p.lim_table = (batch - 1) * p.table_b + tokens * pairs;
+  const void* xs[2] = {a.q, a.k};
+  const void* gs[2] = {a.dq, a.dk};
+  void* os[2] = {a.oq, a.ok};
+  const void* ws[2] = {qw, kw};
+  const int64_t* xst[2] = {a.q_strides, a.k_strides};
+  const int64_t* gst[2] = {a.dq_strides, a.dk_strides};
+  const int64_t* ost[2] = {a.oq_strides, a.ok_strides};
+  const int heads[2] = {hq, hk};
+  const bool inter = interleaved != 0;
+  bool vec = dim % 8 == 0 && dim <= 256 && pairs % 4 == 0 && (reinterpret_cast<uintptr_t>(table) & 15) == 0 &&
+             table_batch_stride % 4 == 0;
+  for (int i = 0; i < 2; ++i) {
+    HeadSide& sd = p.side[i];
+    sd.heads = heads[i];
+    if (heads[i] == 0) continue;
+    sd.x = xs[i];
+    sd.dy = gs[i];
+    sd.y = os[i];
+    sd.w = ws[i];
+    sd.x_b = xst[i][0]; sd.x_l = xst[i][1]; sd.x_h = xst[i][2];
+    sd.y_b = ost[i][0]; sd.y_l = ost[i][1]; sd.y_h = ost[i][2];
+    sd.lim_x = reach(batch, sd.x_b, tokens, sd.x_l, heads[i], sd.x_h, dim);
+    sd.lim_y = reach(batch, sd.y_b, tokens, sd.y_l, heads[i], sd.y_h, dim);
+    vec = vec && head_rows_aligned(sd.x, sd.x_b, sd.x_l, sd.x_h, dtype, inter) &&
+          head_rows_aligned(sd.y, sd.y_b, sd.y_l, sd.y_h, dtype, inter);
+    if (a.back) {
+      sd.dy_b = gst[i][0]; sd.dy_l = gst[i][1]; sd.dy_h = gst[i][2];
+      sd.lim_dy = reach(batch, sd.dy_b, tokens, sd.dy_l, heads[i], sd.dy_h, dim);
+      vec = vec && head_rows_aligned(sd.dy, sd.dy_b, sd.dy_l, sd.dy_h, dtype, inter);
+    }
+  }
+  // A warp's share of a token's heads: all of q or of k where there are tokens enough to fill the machine
+  // (about 32 warps on each SM), else as few as one set of unrolled rows.
+  const int step = std::max(1, 32 / lanes_per_row(dim)) * (a.back ? 2 : 4);
+  int per_warp = std::max(hq, hk);
+  const long long warps = 32ll * sm_count();
+  while (per_warp > step && rows * ((hq + per_warp - 1) / per_warp + (hk + per_warp - 1) / per_warp) < warps)
+    per_warp = std::max(step, (per_warp + 1) / 2);
+  p.heads_per_warp = per_warp;
+  for (int i = 0; i < 2; ++i) p.side[i].chunks = (heads[i] + per_warp - 1) / per_warp;
+  unsigned grid = 0;
+  if (a.back) {
+    const size_t need = bwd_workspace(rows, hq, hk, dim);
+    if (workspace == nullptr || workspace_bytes < need) {
+      set_error("%s: workspace too small: need %zu bytes", a.what, need);
+      return QLIN_EINVAL;
+    }
+    plan_bwd(rows, hq, hk, kBwdRowsPerCta, p.ctas);
+    if (a.dqw != nullptr) p.side[0].dw = reinterpret_cast<float*>(workspace);
+    if (a.dkw != nullptr) p.side[1].dw = reinterpret_cast<float*>(workspace) + (size_t)p.ctas[0] * dim;
+    grid = (unsigned)(p.ctas[0] + p.ctas[1]);
+  } else if (vec) {
+    const long long items = rows * (p.side[0].chunks + p.side[1].chunks);
+    if ((items + 7) / 8 > 0x7fffffff) {
+      set_error("%s: too many rows", a.what);
+      return QLIN_EINVAL;
+    }
+    grid = (unsigned)((items + 7) / 8);
+  } else {
+    for (int i = 0; i < 2; ++i)
+      p.ctas[i] = (int)std::min<long long>(8ll * sm_count(), (rows * heads[i] + 7) / 8);
+    grid = (unsigned)(p.ctas[0] + p.ctas[1]);
+  }
+  if (dtype == QLIN_F16) launch_dtype<QLIN_F16>(p, vec, a.back, grid, stream);
+  else if (dtype == QLIN_BF16) launch_dtype<QLIN_BF16>(p, vec, a.back, grid, stream);
+  else launch_dtype<QLIN_F32>(p, vec, a.back, grid, stream);
+  int rc = rot_launched(a.what);
+  if (rc || !a.back || (a.dqw == nullptr && a.dkw == nullptr)) return rc;
+  DwParams d{};
+  d.part[0] = p.side[0].dw;
+  d.part[1] = p.side[1].dw;
+  d.ctas[0] = p.ctas[0];
+  d.ctas[1] = p.ctas[1];
+  d.out[0] = a.dqw;
+  d.out[1] = a.dkw;
+  d.D = dim;
+  d.w_dtype = w_dtype;
+  dw_sum_kernel<<<dim3((dim + 31) / 32, 2), dim3(32, 32), 0, stream>>>(d);
+  return rot_launched(a.what);
+}
+
+// This translation unit's bounds record (QLIN_CHECKS build).
+QLIN_BOUNDS_READER(bounds_read_rotary)
+
+}  // namespace qlin
+
+using namespace qlin;
+
+extern "C" {
+
+int qlin_rotary_table(const void* positions, int pos_dtype, int64_t tokens, int axes, const int32_t* axes_dim,
+                      double theta, float* table, void* stream) {
+  if (tokens < 0 || axes <= 0 || axes_dim == nullptr || !(theta > 0.0) || !std::isfinite(theta)) {
+    set_error("qlin_rotary_table: bad sizes tokens=%lld axes=%d theta=%g", (long long)tokens, axes, theta);
+    return QLIN_EINVAL;
+  }
+  RotTableParams p;
+  int pairs = 0;
+  for (int a = 0; a < axes; ++a) {
+    if (axes_dim[a] < 0 || axes_dim[a] % 2 != 0) {
+      set_error("qlin_rotary_table: axis %d has %d dimensions (an even number is needed)", a, (int)axes_dim[a]);
+      return QLIN_EINVAL;
+    }
+    if (axes > 256 || axes_dim[a] / 2 > kMaxPairs - pairs) {
+      set_error("qlin_rotary_table: at most %d rotated pairs", kMaxPairs);
+      return QLIN_EDECLINE;
+    }
+    for (int i = 0; i < axes_dim[a] / 2; ++i, ++pairs) {
+      p.turns[pairs] = std::pow(theta, -2.0 * i / axes_dim[a]) * 0.15915494309189533577;  // 1 / (2 pi)
+      p.axis[pairs] = (unsigned char)a;
+    }
+  }
+  if (pos_dtype != QLIN_F32 && pos_dtype != QLIN_I32 && pos_dtype != QLIN_I64) {
+    set_error("qlin_rotary_table: positions are f32, i32 or i64");
+    return QLIN_EDECLINE;
+  }
+  if (tokens == 0 || pairs == 0) return QLIN_OK;
+  if (positions == nullptr || table == nullptr || (reinterpret_cast<uintptr_t>(table) & 7)) {
+    set_error("qlin_rotary_table: null or misaligned pointer");
+    return QLIN_EINVAL;
+  }
+  p.pos = positions;
+  p.tokens = tokens;
+  p.axes = axes;
+  p.pairs = pairs;
+  p.out = reinterpret_cast<float2*>(table);
+  const dim3 block(32, 8), grid((unsigned)std::min<long long>((tokens + 7) / 8, 8ll * sm_count()), (pairs + 31) / 32);
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (pos_dtype == QLIN_F32) rotary_table_kernel<QLIN_F32><<<grid, block, 0, s>>>(p);
+  else if (pos_dtype == QLIN_I32) rotary_table_kernel<QLIN_I32><<<grid, block, 0, s>>>(p);
+  else rotary_table_kernel<QLIN_I64><<<grid, block, 0, s>>>(p);
+  return rot_launched("qlin_rotary_table");
+}
+
+int qlin_qk_norm_rotary(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, int dtype,
+                        int64_t batch, int64_t tokens, int q_heads, int k_heads, int head_dim, const void* q_weight,
+                        const void* k_weight, int weight_dtype, const float* table, int64_t table_batch_stride,
+                        int pairs, float eps, int interleaved, void* q_out, const int64_t* q_out_strides, void* k_out,
+                        const int64_t* k_out_strides, void* stream) {
+  HeadCall a{};
+  a.what = "qlin_qk_norm_rotary";
+  a.q = q;
+  a.k = k;
+  a.q_strides = q_strides;
+  a.k_strides = k_strides;
+  a.oq = q_out;
+  a.ok = k_out;
+  a.oq_strides = q_out_strides;
+  a.ok_strides = k_out_strides;
+  if ((q_heads > 0 && (q_strides == nullptr || q_out_strides == nullptr)) ||
+      (k_heads > 0 && (k_strides == nullptr || k_out_strides == nullptr))) {
+    set_error("%s: null strides", a.what);
+    return QLIN_EINVAL;
+  }
+  return head_norm(a, dtype, batch, tokens, q_heads, k_heads, head_dim, q_weight, k_weight, weight_dtype, table,
+                   table_batch_stride, pairs, eps, interleaved, nullptr, 0, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t qlin_qk_norm_rotary_backward_workspace(int64_t batch, int64_t tokens, int q_heads, int k_heads, int head_dim) {
+  if (batch <= 0 || tokens <= 0 || q_heads < 0 || k_heads < 0 || q_heads + k_heads == 0 || head_dim <= 0) return 0;
+  return bwd_workspace(batch * tokens, q_heads, k_heads, head_dim);
+}
+
+int qlin_qk_norm_rotary_backward(const void* dq, const int64_t* dq_strides, const void* dk, const int64_t* dk_strides,
+                                 const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides,
+                                 int dtype, int64_t batch, int64_t tokens, int q_heads, int k_heads, int head_dim,
+                                 const void* q_weight, const void* k_weight, int weight_dtype, const float* table,
+                                 int64_t table_batch_stride, int pairs, float eps, int interleaved, void* q_grad,
+                                 const int64_t* q_grad_strides, void* k_grad, const int64_t* k_grad_strides,
+                                 void* q_weight_grad, void* k_weight_grad, void* workspace, size_t workspace_bytes,
+                                 void* stream) {
+  HeadCall a{};
+  a.what = "qlin_qk_norm_rotary_backward";
+  a.back = true;
+  a.q = q;
+  a.k = k;
+  a.dq = dq;
+  a.dk = dk;
+  a.q_strides = q_strides;
+  a.k_strides = k_strides;
+  a.dq_strides = dq_strides;
+  a.dk_strides = dk_strides;
+  a.oq = q_grad;
+  a.ok = k_grad;
+  a.oq_strides = q_grad_strides;
+  a.ok_strides = k_grad_strides;
+  a.dqw = q_weight_grad;
+  a.dkw = k_weight_grad;
+  if ((q_heads > 0 && (q_strides == nullptr || dq_strides == nullptr || q_grad_strides == nullptr)) ||
+      (k_heads > 0 && (k_strides == nullptr || dk_strides == nullptr || k_grad_strides == nullptr))) {
+    set_error("%s: null strides", a.what);
+    return QLIN_EINVAL;
+  }
+  return head_norm(a, dtype, batch, tokens, q_heads, k_heads, head_dim, q_weight, k_weight, weight_dtype, table,
+                   table_batch_stride, pairs, eps, interleaved, workspace, workspace_bytes,
+                   reinterpret_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

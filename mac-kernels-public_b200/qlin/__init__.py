@@ -8,6 +8,9 @@ Python signatures follow the reference's callers (roblennon/mac-kernels-public):
   quantize_int8_rowwise  modal/weight_error_app.py:109-115 (activation quantizer of the A8 formats)
   int8_linear_grad_input, w4a8_linear_grad_input, int8_linear_trainable, w4a8_linear_trainable
                        bench/bench_int8_backward.py:52,70, bench/probe_packed_backward_real_k.py:151-158
+and the operators around them that the reference does not have:
+  fp8_linear, fp8_linear_grad_input, fp8_linear_trainable, quantize_fp8_rowwise   block-scaled e4m3 weights
+  rotary_table, qk_norm_rotary, qk_norm_rotary_backward, qk_norm_rotary_trainable  positions, head norms
 
 Every op runs the CUDA library (libqlin.so, sm_100a) on the tensors' device and the current
 stream.  There is no CPU or eager fallback: unsupported inputs raise `QlinDecline`
@@ -26,7 +29,9 @@ from ._lib import QlinDecline, QlinError, check, lib
 __all__ = ["int8_linear", "int8_linear_streamed", "gguf_linear", "gguf_linear_slabs", "gguf_linear_allgather", "peer_wait", "dequantize_gguf", "w4a8_linear", "w4a8_int8_linear", "dequantize_w4a8_int8_weight",
            "quantize_int8_rowwise", "prologue_f16", "repack_gguf", "GGUF_TYPES", "QlinDecline", "QlinError",
            "device_status", "bounds_check", "int8_linear_grad_input", "w4a8_linear_grad_input", "int8_linear_trainable",
-           "w4a8_linear_trainable"]
+           "w4a8_linear_trainable", "fp8_linear", "fp8_linear_grad_input", "fp8_linear_trainable",
+           "quantize_fp8_rowwise", "rotary_table", "qk_norm_rotary", "qk_norm_rotary_backward",
+           "qk_norm_rotary_trainable"]
 
 # ggml type id -> (name, values per block, bytes per block)
 GGUF_TYPES = {2: ("Q4_0", 32, 18), 3: ("Q4_1", 32, 20), 6: ("Q5_0", 32, 22), 7: ("Q5_1", 32, 24),
@@ -81,6 +86,8 @@ SITE_NAMES = {
     13: "int8 gemm shared memory", 14: "small-M weights", 15: "small-M activations", 16: "small-M output/bias/scale",
     17: "prologue input", 18: "prologue output", 19: "repack/decode source", 20: "repack/decode destination",
     21: "split-K finalize", 22: "LoRA packing", 23: "gradient kernels", 24: "kitchen grid", 25: "peer flags",
+    26: "fp8 row quantizer", 27: "fp8 gemm scale/bias", 28: "fp8 gemm output", 29: "fp8 gemm shared memory",
+    30: "fp8 small-M activations", 31: "rotary/head norm input", 32: "rotary/head norm output",
 }
 
 
@@ -416,3 +423,8 @@ def dequantize_w4a8_int8_weight(*args, **kwargs):
 # ---------------------------------------------------------------------------------------------- gradients
 from ._grad import (int8_linear_grad_input, int8_linear_trainable, w4a8_linear_grad_input,  # noqa: E402
                     w4a8_linear_trainable)
+
+# ---------------------------------------------------------------------------------------------- 8-bit floats, attention input
+from ._fp8 import fp8_linear, fp8_linear_grad_input, fp8_linear_trainable, quantize_fp8_rowwise  # noqa: E402
+from ._rotary import (qk_norm_rotary, qk_norm_rotary_backward, qk_norm_rotary_trainable,  # noqa: E402
+                      rotary_table)

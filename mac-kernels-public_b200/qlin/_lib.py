@@ -71,6 +71,18 @@ SIGNATURES = {
     "qlin_w4a8_linear_workspace": (_sz, [_i64, _i64, _i64, _i]),
     "qlin_w4a8_linear": (_i, [_p, _i, _i64, _i64, _i64, _p, _i, _i, _i64, _p, _i, _i, _p, _i, _p, _i, _i64, _p, _sz,
                               _p]),
+    "qlin_fp8_linear_workspace": (_sz, [_i64, _i64, _i64]),
+    "qlin_fp8_linear": (_i, [_p, _i, _i64, _i64, _i64, _p, _i64, _i64, _p, _i64, _p, _i, _p, _i, _i64, _p, _sz, _p]),
+    "qlin_fp8_linear_grad_input_workspace": (_sz, [_i64, _i64, _i64]),
+    "qlin_fp8_linear_grad_input": (_i, [_p, _i, _i64, _i64, _i64, _p, _i64, _i64, _p, _i64, _p, _i, _i64, _p, _sz,
+                                        _p]),
+    "qlin_quantize_rows_fp8": (_i, [_p, _i, _i64, _i64, _i64, _p, _i64, _p, _i64, _p]),
+    "qlin_rotary_table": (_i, [_p, _i, _i64, _i, _p, ctypes.c_double, _p, _p]),
+    "qlin_qk_norm_rotary": (_i, [_p, _p, _p, _p, _i, _i64, _i64, _i, _i, _i, _p, _p, _i, _p, _i64, _i, ctypes.c_float,
+                                 _i, _p, _p, _p, _p, _p]),
+    "qlin_qk_norm_rotary_backward_workspace": (_sz, [_i64, _i64, _i, _i, _i]),
+    "qlin_qk_norm_rotary_backward": (_i, [_p, _p, _p, _p, _p, _p, _p, _p, _i, _i64, _i64, _i, _i, _i, _p, _p, _i, _p,
+                                          _i64, _i, ctypes.c_float, _i, _p, _p, _p, _p, _p, _p, _p, _sz, _p]),
 }
 
 for _name, (_res, _args) in SIGNATURES.items():
@@ -80,7 +92,8 @@ for _name, (_res, _args) in SIGNATURES.items():
         _fn.argtypes = _args
 
 STATUS = {0: "QLIN_OK", 1: "QLIN_EDECLINE", 2: "QLIN_EINVAL", 3: "QLIN_ECUDA", 4: "QLIN_ETIMEOUT"}
-DTYPE_CODE = {"float32": 0, "float16": 1, "bfloat16": 2, "int8": 3, "uint8": 4, "int32": 5, "float8_e4m3fn": 6}
+DTYPE_CODE = {"float32": 0, "float16": 1, "bfloat16": 2, "int8": 3, "uint8": 4, "int32": 5, "float8_e4m3fn": 6,
+              "int64": 7}
 
 
 class QlinError(RuntimeError):
