@@ -2,12 +2,13 @@
 // C ABI (include/qlin.h).
 #include <cuda.h>
 #include <cuda_runtime.h>
-#include <cuda_fp8.h>
 
 #include <algorithm>
 
 #include "../../include/qlin.h"
 #include "qlin_fp8.cuh"
+#include "qlin_fp8_quant.cuh"
+#include "qlin_fp8_small.cuh"
 #include "qlin_internal.h"
 
 namespace qlin {
@@ -23,9 +24,6 @@ namespace qlin {
 // to a lane, with all its loads issued before the first reduction; the 8 scales of a block, which lie
 // side by side in the block-major scale array, go out as one 32-byte piece.
 // ---------------------------------------------------------------------------------------------
-constexpr float kE4m3Max = 448.f;
-constexpr uint32_t kAmaxFloorBits = (127 - 100) << 23;  // 2^-100
-
 struct QuantFp8Params {
   const void* x;
   long long ldx;
@@ -37,60 +35,6 @@ struct QuantFp8Params {
   long long ld_scale;
   long long lim_x, lim_q, lim_scale;  // element counts for the QLIN_CHECKS build
 };
-
-template <int DT>
-__device__ __forceinline__ float load_elem(const void* x, long long i) {
-  if constexpr (DT == QLIN_F16) return __half2float(reinterpret_cast<const __half*>(x)[i]);
-  else if constexpr (DT == QLIN_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(x)[i]);
-  else return reinterpret_cast<const float*>(x)[i];
-}
-
-// 8 consecutive values as stored: 16 bytes of a 2-byte type, 32 of fp32.
-template <int DT>
-struct Raw8 {
-  uint4 v[DT == QLIN_F32 ? 2 : 1];
-};
-
-template <int DT>
-__device__ __forceinline__ Raw8<DT> load_raw8(const void* x, long long i) {
-  Raw8<DT> r;
-  constexpr int kBytes = DT == QLIN_F32 ? 4 : 2;
-  const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(x) + i * kBytes);
-  r.v[0] = __ldg(p);
-  if constexpr (DT == QLIN_F32) r.v[1] = __ldg(p + 1);
-  return r;
-}
-
-template <int DT>
-__device__ __forceinline__ void raw8_to_float(const Raw8<DT>& r, float (&f)[8]) {
-  const uint32_t w[4] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w};
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if constexpr (DT == QLIN_F32) {
-      f[j] = __uint_as_float(w[j]);
-    } else if constexpr (DT == QLIN_F16) {
-      const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
-      f[2 * j] = t.x;
-      f[2 * j + 1] = t.y;
-    } else {
-      f[2 * j] = __uint_as_float(w[j] << 16);
-      f[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-    }
-  }
-  if constexpr (DT == QLIN_F32) {
-    f[4] = __uint_as_float(r.v[1].x);
-    f[5] = __uint_as_float(r.v[1].y);
-    f[6] = __uint_as_float(r.v[1].z);
-    f[7] = __uint_as_float(r.v[1].w);
-  }
-}
-
-// 4 values times r in e4m3, the first in the low byte.
-__device__ __forceinline__ uint32_t to_e4m3x4(float a, float b, float c, float d, float r) {
-  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a * r, b * r), __NV_SATFINITE, __NV_E4M3);
-  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c * r, d * r), __NV_SATFINITE, __NV_E4M3);
-  return lo | (hi << 16);
-}
 
 template <int DT, bool kVec>
 __global__ void __launch_bounds__(256) quant_rows_fp8_kernel(const QuantFp8Params p) {
@@ -120,17 +64,30 @@ __global__ void __launch_bounds__(256) quant_rows_fp8_kernel(const QuantFp8Param
         f[i][j] = (i < rows && c + j < p.K && qchk(BS_FP8_QUANT, at, p.lim_x)) ? load_elem<DT>(p.x, at) : 0.f;
       }
   }
-  float mine = 0.f;  // the scale this lane writes: row lane & 15
+  // Each of the 16 lanes ends up with the maximum of one of the 8 rows (two lanes to a row): at every
+  // step a lane hands the half of its rows to its partner that it does not keep.
+  uint32_t a[kRows];
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
-    uint32_t a = kAmaxFloorBits;
+    a[i] = kAmaxFloorBits;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) a = max(a, __float_as_uint(f[i][j]) & 0x7fffffffu);
+    for (int j = 0; j < 8; ++j) a[i] = max(a[i], __float_as_uint(f[i][j]) & 0x7fffffffu);
+  }
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
-    const float amax = __uint_as_float(a);
-    const float r = __fdiv_rn(kE4m3Max, amax);
-    if ((lane & 15) == i) mine = __fdiv_rn(amax, kE4m3Max);
+  for (int o = 8, n = 4; o > 1; o >>= 1, n >>= 1) {
+    const bool up = lane & o;
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const uint32_t give = up ? a[i] : a[i + n], keep = up ? a[i + n] : a[i];
+      a[i] = max(keep, __shfl_xor_sync(0xffffffffu, give, o));
+    }
+  }
+  a[0] = max(a[0], __shfl_xor_sync(0xffffffffu, a[0], 1));
+  const float amax = __uint_as_float(a[0]);  // of row (lane >> 1) & 7
+  const float up = __fdiv_rn(kE4m3Max, amax);
+#pragma unroll
+  for (int i = 0; i < kRows; ++i) {
+    const float r = __shfl_sync(0xffffffffu, up, (lane & 16) | (i << 1));
     if (i < rows && b < p.kb) {
       const long long at = (long long)(m0 + i) * p.ldq + c;
       if (qchk_span(BS_FP8_QUANT, at, 8, p.lim_q))
@@ -138,9 +95,10 @@ __global__ void __launch_bounds__(256) quant_rows_fp8_kernel(const QuantFp8Param
                                                          to_e4m3x4(f[i][4], f[i][5], f[i][6], f[i][7], r));
     }
   }
-  if ((lane & 15) < rows && b < p.kb) {
-    const long long at = (long long)b * p.ld_scale + m0 + (lane & 15);
-    if (qchk(BS_FP8_QUANT, at, p.lim_scale)) p.scale[at] = mine;
+  const int row = (lane >> 1) & 7;
+  if ((lane & 1) == 0 && row < rows && b < p.kb) {
+    const long long at = (long long)b * p.ld_scale + m0 + row;
+    if (qchk(BS_FP8_QUANT, at, p.lim_scale)) p.scale[at] = __fdiv_rn(amax, kE4m3Max);
   }
 }
 
@@ -186,7 +144,8 @@ static int launch_quant_rows_fp8(const void* x, int x_dtype, long long ldx, int 
 // GEMM launch
 // ---------------------------------------------------------------------------------------------
 template <int CTAS, int TN, bool kTrans>
-static int launch_fp8(const CUtensorMap& tx, const CUtensorMap& tw, const Fp8Params& p, cudaStream_t stream) {
+static int launch_fp8(const CUtensorMap& tx, const CUtensorMap& tw, const CUtensorMap& ty, const Fp8Params& p,
+                      cudaStream_t stream) {
   using Cfg = Fp8Cfg<CTAS, TN>;
   static_assert(Cfg::kSmem <= 232448, "shared memory per CTA");
   auto kern = fp8_gemm_kernel<CTAS, TN, kTrans>;
@@ -213,7 +172,7 @@ static int launch_fp8(const CUtensorMap& tx, const CUtensorMap& tw, const Fp8Par
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tx, tw, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tx, tw, ty, p);
   if (e != cudaSuccess) {
     set_error("fp8 gemm launch failed: %s", cudaGetErrorString(e));
     return QLIN_ECUDA;
@@ -221,11 +180,67 @@ static int launch_fp8(const CUtensorMap& tx, const CUtensorMap& tw, const Fp8Par
   return QLIN_OK;
 }
 
+template <int TN, bool kTrans, int DT>
+static int launch_fp8_small(const CUtensorMap& tw, const Fp8SmallParams& p, cudaStream_t stream) {
+  using Cfg = Fp8SmallCfg<TN>;
+  auto kern = fp8_small_kernel<TN, kTrans, DT>;
+  static bool attr_done[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && !attr_done[dev]) {
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::kSmem) != cudaSuccess) {
+      set_error("cudaFuncSetAttribute(max dynamic smem %d) failed", Cfg::kSmem);
+      return QLIN_ECUDA;
+    }
+    attr_done[dev] = true;
+  }
+  // CTAs that share a tile's contraction: as many (up to 8, a block each at least) as the machine takes at once.
+  const int tiles = (p.N + 127) / 128;
+  const int at_once = sm_count() * Cfg::kCtas;
+  int splits = 1;
+  while (splits < 8 && splits * 2 <= p.kb && tiles * splits * 2 <= at_once) splits *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(tiles * splits));
+  cfg.blockDim = dim3(Cfg::kThreads);
+  cfg.dynamicSmemBytes = Cfg::kSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)splits;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tw, p, splits);
+  if (e != cudaSuccess) {
+    set_error("fp8 small-M launch failed: %s", cudaGetErrorString(e));
+    return QLIN_ECUDA;
+  }
+  return QLIN_OK;
+}
+
+template <int TN, bool kTrans>
+static int small_of_dtype(int x_dtype, const CUtensorMap& tw, const Fp8SmallParams& p, cudaStream_t stream) {
+  if (x_dtype == QLIN_F16) return launch_fp8_small<TN, kTrans, QLIN_F16>(tw, p, stream);
+  if (x_dtype == QLIN_BF16) return launch_fp8_small<TN, kTrans, QLIN_BF16>(tw, p, stream);
+  return launch_fp8_small<TN, kTrans, QLIN_F32>(tw, p, stream);
+}
+
+template <bool kTrans>
+static int run_fp8_small(int x_dtype, const CUtensorMap& tw, const Fp8SmallParams& p, cudaStream_t stream) {
+  if (p.M <= 16) return small_of_dtype<16, kTrans>(x_dtype, tw, p, stream);
+  if (p.M <= 32) return small_of_dtype<32, kTrans>(x_dtype, tw, p, stream);
+  return small_of_dtype<64, kTrans>(x_dtype, tw, p, stream);
+}
+
+// Up to this many tokens the small-M kernel runs, which quantizes them itself and needs no workspace.
+constexpr int64_t kSmallM = 64;
+
 static size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
 
 // Workspace: the e4m3 activations [m, round_up(depth, 128)] and their scales [blocks][m].
 static size_t fp8_workspace(int64_t m, int64_t depth) {
-  if (m <= 0 || depth <= 0) return 0;
+  if (m <= kSmallM || depth <= 0) return 0;
   const int64_t kb = (depth + 127) / 128;
   return align256((size_t)m * kb * 128) + align256((size_t)kb * m * 4);
 }
@@ -275,6 +290,40 @@ static int fp8_product(const char* what, const void* x, int x_dtype, int64_t m, 
   }
   const int kb = (int)((depth + 127) / 128);
   const int64_t kp = (int64_t)kb * 128;
+  const int esz = y_dtype == QLIN_F32 ? 4 : 2;
+  const int y_kind = y_dtype == QLIN_F32 ? OUT_F32 : y_dtype == QLIN_F16 ? OUT_F16 : OUT_BF16;
+  const int64_t sw_out = trans ? 1 : ld_scale, sw_red = trans ? ld_scale : 1;
+  const int64_t lim_sw = ((rows + 127) / 128 - 1) * ld_scale + (cols + 127) / 128;
+  CUtensorMap tx{}, tw{}, ty{};
+  if (kb > 0) {
+    const int rc = make_tmap_2d(&tw, q, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)cols, (uint64_t)rows,
+                                rows > 1 ? (uint64_t)ldq : (uint64_t)cols, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc) return rc;
+  }
+  if (m <= kSmallM && kb > 0) {
+    Fp8SmallParams p{};
+    p.x = x;
+    p.x_dtype = x_dtype;
+    p.x_vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (m == 1 || (ldx * (x_dtype == QLIN_F32 ? 4 : 2)) % 16 == 0);
+    p.ldx = ldx;
+    p.M = (int)m;
+    p.N = (int)out;
+    p.K = (int)depth;
+    p.kb = kb;
+    p.sw = scale;
+    p.sw_out = sw_out;
+    p.sw_red = sw_red;
+    p.bias = bias;
+    p.bias_kind = bk;
+    p.y = y;
+    p.y_dtype = y_kind;
+    p.ldy = ldy;
+    p.status = reinterpret_cast<DeviceStatus*>(device_status_ptr());
+    p.lim_x = (m - 1) * ldx + depth;
+    p.lim_y = (m - 1) * ldy + out;
+    p.lim_sw = lim_sw;
+    return trans ? run_fp8_small<true>(x_dtype, tw, p, stream) : run_fp8_small<false>(x_dtype, tw, p, stream);
+  }
   uint8_t* xq = reinterpret_cast<uint8_t*>(workspace);
   float* sx = reinterpret_cast<float*>(xq + align256((size_t)m * kp));
   Fp8Params p{};
@@ -284,19 +333,18 @@ static int fp8_product(const char* what, const void* x, int x_dtype, int64_t m, 
   p.sx = sx;
   p.ld_sx = m;
   p.sw = scale;
-  p.sw_out = trans ? 1 : ld_scale;
-  p.sw_red = trans ? ld_scale : 1;
+  p.sw_out = sw_out;
+  p.sw_red = sw_red;
   p.bias = bias;
   p.bias_kind = bk;
   p.y = y;
-  p.y_dtype = y_dtype == QLIN_F32 ? OUT_F32 : y_dtype == QLIN_F16 ? OUT_F16 : OUT_BF16;
+  p.y_dtype = y_kind;
   p.ldy = ldy;
-  const int esz = y_dtype == QLIN_F32 ? 4 : 2;
-  p.vec_out = (reinterpret_cast<uintptr_t>(y) & 15) == 0 && (ldy * esz) % 16 == 0;
+  p.tma_out = (reinterpret_cast<uintptr_t>(y) & 15) == 0 && (ldy * esz) % 16 == 0;
   p.status = reinterpret_cast<DeviceStatus*>(device_status_ptr());
   p.lim_y = (m - 1) * ldy + out;
   p.lim_sx = (long long)kb * m;
-  p.lim_sw = (long long)((rows + 127) / 128 - 1) * ld_scale + (cols + 127) / 128;
+  p.lim_sw = lim_sw;
   const bool pair = m > 128 && out > 128;
   const int64_t m_tiles = (m + 127) / 128, n_tiles = (out + 127) / 128;
   if (m_tiles * n_tiles > 0x7fffffff) {
@@ -305,19 +353,23 @@ static int fp8_product(const char* what, const void* x, int x_dtype, int64_t m, 
   }
   p.m_tiles = (int)(pair ? (m_tiles + 1) / 2 : m_tiles);
   p.n_tiles = (int)(pair ? (n_tiles + 1) / 2 : n_tiles);
-  CUtensorMap tx{}, tw{};
+  if (p.tma_out) {
+    const int rc = make_tmap_2d(&ty, y, y_dtype == QLIN_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                        : y_dtype == QLIN_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                              : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                                esz, (uint64_t)out, (uint64_t)m, (uint64_t)ldy * esz, 128 / esz, 32,
+                                CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc) return rc;
+  }
   if (kb > 0) {
     int rc = launch_quant_rows_fp8(x, x_dtype, ldx, (int)m, (int)depth, xq, kp, sx, m, stream);
     if (rc) return rc;
     rc = make_tmap_2d(&tx, xq, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)kp, (uint64_t)m, (uint64_t)kp, 128, 128,
                       CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc) return rc;
-    rc = make_tmap_2d(&tw, q, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (uint64_t)cols, (uint64_t)rows,
-                      rows > 1 ? (uint64_t)ldq : (uint64_t)cols, 128, 128, CU_TENSOR_MAP_SWIZZLE_128B);
-    if (rc) return rc;
   }
-  if (pair) return trans ? launch_fp8<2, 256, true>(tx, tw, p, stream) : launch_fp8<2, 256, false>(tx, tw, p, stream);
-  return trans ? launch_fp8<1, 128, true>(tx, tw, p, stream) : launch_fp8<1, 128, false>(tx, tw, p, stream);
+  if (pair) return trans ? launch_fp8<2, 256, true>(tx, tw, ty, p, stream) : launch_fp8<2, 256, false>(tx, tw, ty, p, stream);
+  return trans ? launch_fp8<1, 128, true>(tx, tw, ty, p, stream) : launch_fp8<1, 128, false>(tx, tw, ty, p, stream);
 }
 
 // This translation unit's bounds record (QLIN_CHECKS build).

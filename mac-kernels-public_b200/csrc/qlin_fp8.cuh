@@ -12,11 +12,15 @@
 // cores fill the next buffer.  Tokens lie on the TMEM lanes: a thread owns one token, whose scale times
 // the warp's block scale is one factor for all of its values.
 //
-// Warp roles (320 threads, one CTA per SM, persistent over the tiles):
-//   warp 0        TMA producer            warp 1   TMEM alloc + MMA issuer
-//   warps 2..9    rescale + epilogue: two warps per TMEM lane quarter, half the columns each
+// Warp roles (384 threads, one CTA per SM, persistent over the tiles):
+//   warp 0        TMA producer            warp 1   TMEM alloc + MMA issuer       (warps 2, 3 idle)
+//   warps 4..11   rescale + epilogue: two warps per TMEM lane quarter, half the columns each
+// The epilogue warps take over most of the first warpgroup's registers: a pair's warp holds 128 running
+// sums and two loads of 32 values.
 #pragma once
 #include <cuda.h>
+
+#include <type_traits>
 
 #include "qlin_ptx.cuh"
 
@@ -35,7 +39,7 @@ struct Fp8Params {
   void* y;
   int y_dtype;      // OutDType
   long long ldy;
-  int vec_out;      // rows of y take 16-byte stores
+  int tma_out;      // y's rows are 16-byte aligned: the output leaves through tmap_y
   DeviceStatus* status;
   // Element counts of the caller's buffers for the QLIN_CHECKS build (unused otherwise).
   long long lim_y, lim_sx, lim_sw;
@@ -45,14 +49,16 @@ struct Fp8Params {
 // 256 tokens x TN channels, each CTA holding its 128 tokens and half of the channels.
 template <int CTAS, int TN>
 struct Fp8Cfg {
-  static constexpr int kThreads = 320;
+  static constexpr int kEpiWarps = 8;
+  static constexpr int kThreads = 128 + 32 * kEpiWarps;
   static constexpr int kBuf = 512 / TN;        // accumulator buffers in TMEM
   static constexpr int kBRows = TN / CTAS;     // channels this CTA loads per stage
   static constexpr uint32_t kAStage = 128 * 128;
   static constexpr uint32_t kBStage = kBRows * 128;
-  static constexpr int kStages = 6;
-  static constexpr int kCols = TN / 2;         // accumulator columns per epilogue warp
-  static constexpr int kSmem = 1024 + kStages * (int)(kAStage + kBStage) + 512;
+  static constexpr int kStages = 5;
+  static constexpr int kCols = TN / (kEpiWarps / 4);  // accumulator columns per epilogue warp
+  static constexpr uint32_t kOutWarp = 32 * kCols * 2;  // output staging of a warp: its tokens' rows, 2 bytes a value
+  static constexpr int kSmem = 1024 + kStages * (int)(kAStage + kBStage) + kEpiWarps * (int)kOutWarp + 512;
   static_assert(CTAS == 1 || CTAS == 2, "one CTA or a pair");
   static_assert(kBRows == 128, "the transposed operand is one 128-column block");
 };
@@ -97,9 +103,9 @@ __device__ __forceinline__ uint32_t pack_out2(int dtype, float a, float b) {
 }
 
 template <int CTAS, int TN, bool kTrans>
-__global__ void __launch_bounds__(320, 1)
+__global__ void __launch_bounds__(Fp8Cfg<CTAS, TN>::kThreads, 1)
 fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w,
-                const Fp8Params p) {
+                const __grid_constant__ CUtensorMap tmap_y, const Fp8Params p) {
   using Cfg = Fp8Cfg<CTAS, TN>;
   constexpr int STAGES = Cfg::kStages;
   constexpr int NB = Cfg::kBuf;
@@ -107,7 +113,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sa = smem;
   uint8_t* sb = sa + STAGES * Cfg::kAStage;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sb + STAGES * Cfg::kBStage);
+  uint8_t* so = sb + STAGES * Cfg::kBStage;  // 8 x kOutWarp
+  uint64_t* bars = reinterpret_cast<uint64_t*>(so + Cfg::kEpiWarps * Cfg::kOutWarp);
   uint64_t* full = bars;              // [STAGES] both CTAs' operands landed (even CTA's)
   uint64_t* empty = full + STAGES;    // [STAGES] MMAs that read the stage completed (each CTA's)
   uint64_t* acc_full = empty + STAGES;   // [NB] products ready (each CTA's)
@@ -130,7 +137,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
     }
     for (int b = 0; b < NB; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 8 * CTAS);
+      mbar_init(&acc_empty[b], Cfg::kEpiWarps * CTAS);
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -152,6 +159,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
   if (warp == 0 && lane == 0 && p.kb > 0) {
     prefetch_tmap(&tmap_x);
     prefetch_tmap(&tmap_w);
+    if (p.tma_out) prefetch_tmap(&tmap_y);
   }
   tc_fence_before();
   __syncthreads();
@@ -159,92 +167,97 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  if (warp == 0) {
-    // --------------------------------------------------------------------- producer (both CTAs)
-    if (elect_one()) {
-      const uint32_t full_leader = CTAS == 2 ? cluster_map(full, 0) : smem_u32(full);
-      uint32_t it = 0;
-      bool ok = true;
-      for (int t = tile0; t < num_tiles && ok; t += tile_step) {
-        int mt, nt;
-        fp8_tile(t, p.m_tiles, p.n_tiles, mt, nt);
-        const int m0 = (mt * CTAS + (int)rank) * 128;
-        const int n0 = nt * TN + (int)rank * Cfg::kBRows;
-        for (int b = 0; b < p.kb; ++b, ++it) {
-          const int s = it % STAGES;
-          if (!mbar_wait(&empty[s], ((it / STAGES) & 1) ^ 1, abort_flag, p.status, 0x41)) { ok = false; break; }
-          if (rank == 0) mbar_arrive_expect_tx(&full[s], CTAS * (Cfg::kAStage + Cfg::kBStage));
-          const int wx = kTrans ? n0 : b * 128, wy = kTrans ? b * 128 : n0;
-          if constexpr (CTAS == 2) {
-            const uint32_t bar = full_leader + (uint32_t)(s * 8);
-            tma_load_2d_pair(sa + s * Cfg::kAStage, &tmap_x, bar, b * 128, m0);
-            tma_load_2d_pair(sb + s * Cfg::kBStage, &tmap_w, bar, wx, wy);
-          } else {
-            tma_load_2d(sa + s * Cfg::kAStage, &tmap_x, &full[s], b * 128, m0);
-            tma_load_2d(sb + s * Cfg::kBStage, &tmap_w, &full[s], wx, wy);
+  // setmaxnreg: 2 x 224 + 56 = 3 x 168, the registers of an SM quarter's three warps at launch
+  if (warp < 4) {
+    setmaxnreg_dec<56>();
+    if (warp == 0) {
+      // --------------------------------------------------------------------- producer (both CTAs)
+      if (elect_one()) {
+        const uint32_t full_leader = CTAS == 2 ? cluster_map(full, 0) : smem_u32(full);
+        uint32_t it = 0;
+        bool ok = true;
+        for (int t = tile0; t < num_tiles && ok; t += tile_step) {
+          int mt, nt;
+          fp8_tile(t, p.m_tiles, p.n_tiles, mt, nt);
+          const int m0 = (mt * CTAS + (int)rank) * 128;
+          const int n0 = nt * TN + (int)rank * Cfg::kBRows;
+          for (int b = 0; b < p.kb; ++b, ++it) {
+            const int s = it % STAGES;
+            if (!mbar_wait(&empty[s], ((it / STAGES) & 1) ^ 1, abort_flag, p.status, 0x41)) { ok = false; break; }
+            if (rank == 0) mbar_arrive_expect_tx(&full[s], CTAS * (Cfg::kAStage + Cfg::kBStage));
+            const int wx = kTrans ? n0 : b * 128, wy = kTrans ? b * 128 : n0;
+            if constexpr (CTAS == 2) {
+              const uint32_t bar = full_leader + (uint32_t)(s * 8);
+              tma_load_2d_pair(sa + s * Cfg::kAStage, &tmap_x, bar, b * 128, m0);
+              tma_load_2d_pair(sb + s * Cfg::kBStage, &tmap_w, bar, wx, wy);
+            } else {
+              tma_load_2d(sa + s * Cfg::kAStage, &tmap_x, &full[s], b * 128, m0);
+              tma_load_2d(sb + s * Cfg::kBStage, &tmap_w, &full[s], wx, wy);
+            }
+          }
+        }
+        if (!ok && rank == 0) {  // wait for the copies in flight (the even CTA's barriers count both CTAs' bytes)
+          for (uint32_t j = (it >= (uint32_t)STAGES ? it - STAGES : 0); j < it; ++j) {
+            const uint64_t t0 = globaltimer();
+            while (!mbar_try_wait(smem_u32(&full[j % STAGES]), (j / STAGES) & 1)) {
+              if (globaltimer() - t0 > QLIN_WAIT_TIMEOUT_NS) break;
+            }
           }
         }
       }
-      if (!ok && rank == 0) {  // wait for the copies in flight (the even CTA's barriers count both CTAs' bytes)
-        for (uint32_t j = (it >= (uint32_t)STAGES ? it - STAGES : 0); j < it; ++j) {
-          const uint64_t t0 = globaltimer();
-          while (!mbar_try_wait(smem_u32(&full[j % STAGES]), (j / STAGES) & 1)) {
-            if (globaltimer() - t0 > QLIN_WAIT_TIMEOUT_NS) break;
-          }
-        }
-      }
-    }
-  } else if (warp == 1) {
-    // --------------------------------------------------------------------- MMA issuer (even CTA)
-    if (rank == 0 && elect_one()) {
-      constexpr uint32_t idesc = idesc_e4m3_f32(128 * CTAS, TN, false, kTrans);
-      // 32 contraction indices of one MMA: 32 bytes of a K-major row, or 32 rows of a transposed tile
-      constexpr uint64_t kBStep = kTrans ? (32 * 128) >> 4 : 32 >> 4;
-      uint32_t it = 0;
-      bool ok = true;
-      for (int t = tile0; t < num_tiles && ok; t += tile_step) {
-        for (int b = 0; b < p.kb; ++b, ++it) {
-          const int s = it % STAGES;
-          const uint32_t buf = it % NB;
-          if (!mbar_wait<CTAS == 2>(&full[s], (it / STAGES) & 1, abort_flag, p.status, 0x42) ||
-              !mbar_wait<CTAS == 2>(&acc_empty[buf], ((it / NB) & 1) ^ 1, abort_flag, p.status, 0x43)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          const uint64_t a_desc = smem_desc_sw128(smem_u32(sa + s * Cfg::kAStage));
-          const uint32_t sb_u = smem_u32(sb + s * Cfg::kBStage);
-          const uint64_t b_desc = kTrans ? smem_desc_sw128_mn(sb_u) : smem_desc_sw128(sb_u);
+    } else if (warp == 1) {
+      // --------------------------------------------------------------------- MMA issuer (even CTA)
+      if (rank == 0 && elect_one()) {
+        constexpr uint32_t idesc = idesc_e4m3_f32(128 * CTAS, TN, false, kTrans);
+        // 32 contraction indices of one MMA: 32 bytes of a K-major row, or 32 rows of a transposed tile
+        constexpr uint64_t kBStep = kTrans ? (32 * 128) >> 4 : 32 >> 4;
+        uint32_t it = 0;
+        bool ok = true;
+        for (int t = tile0; t < num_tiles && ok; t += tile_step) {
+          for (int b = 0; b < p.kb; ++b, ++it) {
+            const int s = it % STAGES;
+            const uint32_t buf = it % NB;
+            if (!mbar_wait<CTAS == 2>(&full[s], (it / STAGES) & 1, abort_flag, p.status, 0x42) ||
+                !mbar_wait<CTAS == 2>(&acc_empty[buf], ((it / NB) & 1) ^ 1, abort_flag, p.status, 0x43)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint64_t a_desc = smem_desc_sw128(smem_u32(sa + s * Cfg::kAStage));
+            const uint32_t sb_u = smem_u32(sb + s * Cfg::kBStage);
+            const uint64_t b_desc = kTrans ? smem_desc_sw128_mn(sb_u) : smem_desc_sw128(sb_u);
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk) {
-            const uint64_t ad = a_desc + (uint64_t)(kk * 2), bd = b_desc + (uint64_t)kk * kBStep;
-            if constexpr (CTAS == 2) mma_f8_ss_pair(tmem_base + buf * TN, ad, bd, idesc, kk > 0);
-            else mma_f8_ss(tmem_base + buf * TN, ad, bd, idesc, kk > 0);
-          }
-          if constexpr (CTAS == 2) {
-            tc_commit_pair(cluster_map(&acc_full[buf], 0));
-            tc_commit_pair(cluster_map(&acc_full[buf], 1));
-            tc_commit_pair(cluster_map(&empty[s], 0));
-            tc_commit_pair(cluster_map(&empty[s], 1));
-          } else {
-            tc_commit(&acc_full[buf]);
-            tc_commit(&empty[s]);
+            for (int kk = 0; kk < 4; ++kk) {
+              const uint64_t ad = a_desc + (uint64_t)(kk * 2), bd = b_desc + (uint64_t)kk * kBStep;
+              if constexpr (CTAS == 2) mma_f8_ss_pair(tmem_base + buf * TN, ad, bd, idesc, kk > 0);
+              else mma_f8_ss(tmem_base + buf * TN, ad, bd, idesc, kk > 0);
+            }
+            if constexpr (CTAS == 2) {
+              tc_commit_pair(cluster_map(&acc_full[buf], 0));
+              tc_commit_pair(cluster_map(&acc_full[buf], 1));
+              tc_commit_pair(cluster_map(&empty[s], 0));
+              tc_commit_pair(cluster_map(&empty[s], 1));
+            } else {
+              tc_commit(&acc_full[buf]);
+              tc_commit(&empty[s]);
+            }
           }
         }
-      }
-      if constexpr (CTAS == 2) tc_commit_pair(cluster_map(drain, 0));
-      else tc_commit(drain);
-      const uint64_t t0 = globaltimer();
-      while (!mbar_try_wait(smem_u32(drain), 0)) {
-        if (globaltimer() - t0 > QLIN_WAIT_TIMEOUT_NS) break;
+        if constexpr (CTAS == 2) tc_commit_pair(cluster_map(drain, 0));
+        else tc_commit(drain);
+        const uint64_t t0 = globaltimer();
+        while (!mbar_try_wait(smem_u32(drain), 0)) {
+          if (globaltimer() - t0 > QLIN_WAIT_TIMEOUT_NS) break;
+        }
       }
     }
   } else {
+    setmaxnreg_inc<224>();
     // --------------------------------------------------------------------- rescale + epilogue
     constexpr int kCols = Cfg::kCols;
     constexpr int kChunk = 16;
     const int quarter = warp & 3;
-    const int part = (warp - 2) >> 2;
+    const int part = (warp - 4) >> 2;
     const int r = quarter * 32 + lane;  // TMEM lane == token within this CTA's 128
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const uint32_t acc_empty_leader = CTAS == 2 ? cluster_map(acc_empty, 0) : smem_u32(acc_empty);
@@ -255,76 +268,145 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
       fp8_tile(t, p.m_tiles, p.n_tiles, mt, nt);
       const int m = (mt * CTAS + (int)rank) * 128 + r;
       const int n0 = nt * TN + part * kCols;  // kCols channels from here, inside one 128-channel block
-      const bool m_ok = m < p.M;
       const long long sw_off = (long long)min(n0 / 128, (p.N - 1) / 128) * p.sw_out;
-      float acc[kCols];
+      float acc[kCols];  // the sums start from the bias
+      if (p.bias_kind != 0) {
 #pragma unroll
-      for (int j = 0; j < kCols; ++j) acc[j] = 0.f;
-      auto load_sx = [&](int b) {
-        const long long i = (long long)b * p.ld_sx + m;
-        return (m_ok && b < p.kb && qchk(BS_FP8_SCALE, i, p.lim_sx)) ? __ldg(p.sx + i) : 0.f;
-      };
-      auto load_sw = [&](int b) {
-        const long long i = sw_off + (long long)b * p.sw_red;
-        return (b < p.kb && qchk(BS_FP8_SCALE, i, p.lim_sw)) ? __ldg(p.sw + i) : 0.f;
-      };
-      float sx = load_sx(0), sw = load_sw(0);  // the next block's scales are in flight during a block
-      for (int b = 0; b < p.kb; ++b, ++it) {
-        const float s = sx * sw;
-        sx = load_sx(b + 1);
-        sw = load_sw(b + 1);
-        const uint32_t buf = it % NB;
-        if (!mbar_wait(&acc_full[buf], (it / NB) & 1, abort_flag, p.status, 0x44)) { ok = false; break; }
-        tc_fence_after();
-        const uint32_t taddr = tmem_base + lanes + buf * TN + part * kCols;
+        for (int c0 = 0; c0 < kCols; c0 += 32) {
+          const float mine = n0 + c0 + lane < p.N ? fp8_bias(p.bias, p.bias_kind, n0 + c0 + lane, p.N) : 0.f;
 #pragma unroll
-        for (int c0 = 0; c0 < kCols; c0 += kChunk) {
-          uint32_t v[kChunk];
-          tmem_ld16(taddr + c0, v);
-          tmem_wait_ld();
-          if (c0 + kChunk >= kCols) {  // the last values are in registers: the buffer goes back to the issuer
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-              if constexpr (CTAS == 2) mbar_arrive_cluster(acc_empty_leader + buf * 8);
-              else mbar_arrive(&acc_empty[buf]);
+          for (int j = 0; j < 32; ++j) acc[c0 + j] = __shfl_sync(0xffffffffu, mine, j);
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < kCols; ++j) acc[j] = 0.f;
+      }
+      // Scales come from L2, at times from HBM: a token's are asked for kAhead blocks before their use, and
+      // the weight's, one for all lanes, 32 blocks at a time, a lane each.
+      constexpr int kAhead = 4;
+      const float* sx_next = p.sx + min(m, p.M - 1);
+      int left = p.kb - 1;  // blocks after the one sx_next points at
+      auto take_sx = [&]() {
+        const float v = qchk(BS_FP8_SCALE, sx_next - p.sx, p.lim_sx) ? __ldg(sx_next) : 0.f;
+        if (left > 0) sx_next += p.ld_sx;
+        --left;
+        return v;
+      };
+      auto take_sw = [&](int b) {
+        const long long i = sw_off + (long long)min(b + lane, p.kb - 1) * p.sw_red;
+        return qchk(BS_FP8_SCALE, i, p.lim_sw) ? __ldg(p.sw + i) : 0.f;
+      };
+      float sx[kAhead], sw = p.kb > 0 ? take_sw(0) : 0.f;
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) sx[u] = p.kb > 0 ? take_sx() : 0.f;
+      for (int b0 = 0; b0 < p.kb && ok; b0 += kAhead) {
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          const int b = b0 + u;
+          if (b >= p.kb) break;
+          const float s = sx[u] * __shfl_sync(0xffffffffu, sw, b & 31);
+          if ((b & 31) == 31) sw = take_sw(b + 1);
+          sx[u] = take_sx();
+          const uint32_t buf = it % NB;
+          if (!mbar_wait(&acc_full[buf], (it / NB) & 1, abort_flag, p.status, 0x44)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t taddr = tmem_base + lanes + buf * TN + part * kCols;
+          // the next chunk's load is in flight during a chunk's arithmetic
+          uint32_t v[2][kChunk];
+          tmem_ld_cols<kChunk>(taddr, v[0]);
+#pragma unroll
+          for (int c = 0; c < kCols / kChunk; ++c) {
+            tmem_wait_ld_of(v[c & 1]);
+            if (c + 1 < kCols / kChunk) {
+              tmem_ld_cols<kChunk>(taddr + (c + 1) * kChunk, v[(c + 1) & 1]);
+            } else {  // the last values are in registers: the buffer goes back to the issuer
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) {
+                if constexpr (CTAS == 2) mbar_arrive_cluster(acc_empty_leader + buf * 8);
+                else mbar_arrive(&acc_empty[buf]);
+              }
             }
-          }
 #pragma unroll
-          for (int j = 0; j < kChunk; j += 2) ffma2(s, v[j], v[j + 1], acc[c0 + j], acc[c0 + j + 1]);
+            for (int j = 0; j < kChunk; j += 2)
+              ffma2(s, v[c & 1][j], v[c & 1][j + 1], acc[c * kChunk + j], acc[c * kChunk + j + 1]);
+          }
+          ++it;
         }
       }
       if (!ok) break;
-      if (m_ok && n0 < p.N) {
-        const long long row = (long long)m * p.ldy;
+      // The warp's 32 rows go through its own staging buffer, 128 bytes of each row at a time, 16-byte pieces
+      // swizzled by the row; they leave as TMA stores (clipped at M and N), which the next tile's products
+      // do not wait for, or, where y's rows are not 16-byte aligned, as plain stores along the rows.
+      const int m_warp = (mt * CTAS + (int)rank) * 128 + quarter * 32;
+      uint8_t* stage = so + (warp - 4) * Cfg::kOutWarp;
+      constexpr int kPieceBytes = 32 * 128;
+      constexpr int kPieces = Cfg::kOutWarp / kPieceBytes;
+      bool used[kPieces] = {};
+      const bool wide = p.y_dtype == OUT_F32;
+      if (lane == 0) bulk_wait_read<0>();  // the last tile's stores have left the buffer
+      __syncwarp();
+      auto piece = [&](auto wide_c, int c0) {  // 128 bytes of every row: the values from column c0
+        constexpr bool kWide = decltype(wide_c)::value;
+        constexpr int kN = kWide ? 32 : 64;
+        const int slot = (c0 / kN) % kPieces;
+        uint8_t* dst = stage + slot * kPieceBytes;
+        if (used[slot]) {  // fp32 only: the buffer holds half of the row
+          if (lane == 0) bulk_wait_read<0>();
+          __syncwarp();
+        }
+        used[slot] = true;
+        if (qchk_smem(BS_FP8_SMEM, smem_raw, dst, kPieceBytes)) {
 #pragma unroll
-        for (int c0 = 0; c0 < kCols; c0 += 8) {
-          const int n = n0 + c0;
-          float o[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) o[j] = acc[c0 + j] + (n + j < p.N ? fp8_bias(p.bias, p.bias_kind, n + j, p.N) : 0.f);
-          if (p.vec_out && n + 8 <= p.N && qchk_span(BS_FP8_Y, row + n, 8, p.lim_y)) {
-            if (p.y_dtype == OUT_F32) {
-              float4* y = reinterpret_cast<float4*>(reinterpret_cast<float*>(p.y) + row + n);
-              y[0] = make_float4(o[0], o[1], o[2], o[3]);
-              y[1] = make_float4(o[4], o[5], o[6], o[7]);
+          for (int ch = 0; ch < 8; ++ch) {
+            uint4 w;
+            if constexpr (kWide) {
+              w = make_uint4(__float_as_uint(acc[c0 + 4 * ch]), __float_as_uint(acc[c0 + 4 * ch + 1]),
+                             __float_as_uint(acc[c0 + 4 * ch + 2]), __float_as_uint(acc[c0 + 4 * ch + 3]));
             } else {
-              *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(p.y) + row + n) =
-                  make_uint4(pack_out2(p.y_dtype, o[0], o[1]), pack_out2(p.y_dtype, o[2], o[3]),
-                             pack_out2(p.y_dtype, o[4], o[5]), pack_out2(p.y_dtype, o[6], o[7]));
+              w = make_uint4(pack_out2(p.y_dtype, acc[c0 + 8 * ch], acc[c0 + 8 * ch + 1]),
+                             pack_out2(p.y_dtype, acc[c0 + 8 * ch + 2], acc[c0 + 8 * ch + 3]),
+                             pack_out2(p.y_dtype, acc[c0 + 8 * ch + 4], acc[c0 + 8 * ch + 5]),
+                             pack_out2(p.y_dtype, acc[c0 + 8 * ch + 6], acc[c0 + 8 * ch + 7]));
             }
-          } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              if (n + j >= p.N || !qchk(BS_FP8_Y, row + n + j, p.lim_y)) continue;
-              if (p.y_dtype == OUT_F32) reinterpret_cast<float*>(p.y)[row + n + j] = o[j];
-              else if (p.y_dtype == OUT_F16) reinterpret_cast<__half*>(p.y)[row + n + j] = __float2half_rn(o[j]);
-              else reinterpret_cast<__nv_bfloat16*>(p.y)[row + n + j] = __float2bfloat16_rn(o[j]);
-            }
+            *reinterpret_cast<uint4*>(dst + lane * 128 + ((ch ^ (lane & 7)) << 4)) = w;
           }
         }
+        const int n = n0 + c0;
+        if (p.tma_out) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if (n < p.N && m_warp < p.M) tma_store_2d(&tmap_y, dst, n, m_warp);
+            bulk_commit();
+          }
+        } else {
+          __syncwarp();
+          const int rows = min(32, p.M - m_warp);
+          for (int rr = 0; rr < rows; ++rr) {
+#pragma unroll
+            for (int q = 0; q < kN / 32; ++q) {
+              const int j = q * 32 + lane;
+              const int byte = kWide ? j * 4 : j * 2;
+              const uint8_t* src = dst + rr * 128 + ((((byte >> 4) ^ (rr & 7)) << 4) | (byte & 15));
+              const long long at = (long long)(m_warp + rr) * p.ldy + n + j;
+              if (n + j >= p.N || !qchk(BS_FP8_Y, at, p.lim_y)) continue;
+              if constexpr (kWide) reinterpret_cast<float*>(p.y)[at] = *reinterpret_cast<const float*>(src);
+              else reinterpret_cast<uint16_t*>(p.y)[at] = *reinterpret_cast<const uint16_t*>(src);
+            }
+          }
+          __syncwarp();
+        }
+      };
+      if (wide) {
+#pragma unroll
+        for (int c0 = 0; c0 < kCols; c0 += 32) piece(std::true_type{}, c0);
+      } else {
+#pragma unroll
+        for (int c0 = 0; c0 < kCols; c0 += 64) piece(std::false_type{}, c0);
       }
     }
+    if (lane == 0) bulk_wait_all();
   }
 
   // Warps 0 and 1 ran their loops on one elected lane; reconverge before the block barrier

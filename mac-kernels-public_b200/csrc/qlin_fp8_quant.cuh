@@ -1,0 +1,68 @@
+// Bringing rows of f32, f16 or bf16 to e4m3: loads and conversions shared by the row quantizer and the small-M
+// product, which quantizes its few rows itself.
+#pragma once
+#include <cuda_fp8.h>
+
+#include "../../include/qlin.h"
+#include "qlin_ptx.cuh"
+
+namespace qlin {
+
+constexpr float kE4m3Max = 448.f;
+constexpr uint32_t kAmaxFloorBits = (127 - 100) << 23;  // 2^-100
+
+template <int DT>
+__device__ __forceinline__ float load_elem(const void* x, long long i) {
+  if constexpr (DT == QLIN_F16) return __half2float(reinterpret_cast<const __half*>(x)[i]);
+  else if constexpr (DT == QLIN_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(x)[i]);
+  else return reinterpret_cast<const float*>(x)[i];
+}
+
+// 8 consecutive values as stored: 16 bytes of a 2-byte type, 32 of fp32.
+template <int DT>
+struct Raw8 {
+  uint4 v[DT == QLIN_F32 ? 2 : 1];
+};
+
+template <int DT>
+__device__ __forceinline__ Raw8<DT> load_raw8(const void* x, long long i) {
+  Raw8<DT> r;
+  constexpr int kBytes = DT == QLIN_F32 ? 4 : 2;
+  const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(x) + i * kBytes);
+  r.v[0] = __ldg(p);
+  if constexpr (DT == QLIN_F32) r.v[1] = __ldg(p + 1);
+  return r;
+}
+
+template <int DT>
+__device__ __forceinline__ void raw8_to_float(const Raw8<DT>& r, float (&f)[8]) {
+  const uint32_t w[4] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (DT == QLIN_F32) {
+      f[j] = __uint_as_float(w[j]);
+    } else if constexpr (DT == QLIN_F16) {
+      const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+      f[2 * j] = t.x;
+      f[2 * j + 1] = t.y;
+    } else {
+      f[2 * j] = __uint_as_float(w[j] << 16);
+      f[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+    }
+  }
+  if constexpr (DT == QLIN_F32) {
+    f[4] = __uint_as_float(r.v[1].x);
+    f[5] = __uint_as_float(r.v[1].y);
+    f[6] = __uint_as_float(r.v[1].z);
+    f[7] = __uint_as_float(r.v[1].w);
+  }
+}
+
+// 4 values times r in e4m3, the first in the low byte.
+__device__ __forceinline__ uint32_t to_e4m3x4(float a, float b, float c, float d, float r) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a * r, b * r), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c * r, d * r), __NV_SATFINITE, __NV_E4M3);
+  return lo | (hi << 16);
+}
+
+}  // namespace qlin

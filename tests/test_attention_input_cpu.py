@@ -20,7 +20,7 @@ def lib():
 
 
 def test_workspaces(lib):
-    assert lib.qlin_fp8_linear_workspace(0, 64, 128) == 0 and lib.qlin_fp8_linear_workspace(4, 64, 0) == 0
+    assert lib.qlin_fp8_linear_workspace(0, 64, 128) == 0 and lib.qlin_fp8_linear_workspace(64, 64, 128) == 0 and lib.qlin_fp8_linear_workspace(4, 64, 0) == 0
     assert lib.qlin_fp8_linear_workspace(300, 64, 200) >= 300 * 256 + 2 * 300 * 4
     assert lib.qlin_fp8_linear_grad_input_workspace(300, 200, 64) >= 300 * 256 + 2 * 300 * 4
     assert lib.qlin_qk_norm_rotary_backward_workspace(0, 5, 2, 2, 64) == 0
@@ -36,8 +36,8 @@ def _linear(lib, m=4, k=128, ldx=128, ldq=128, n=8, ld_scale=1, x=SOME, q=SOME, 
     (dict(m=-1), 2), (dict(k=-16), 2), (dict(n=-1), 2), (dict(ldx=64), 2), (dict(ldq=112), 2), (dict(ldy=4), 2),
     (dict(n=300, ldy=300, k=256, ldx=256, ldq=256, ld_scale=1), 2), (dict(m=1 << 31), 2), (dict(xd=I32), 1),
     (dict(yd=I32), 1), (dict(bias=SOME, bd=I32), 1), (dict(k=120, ldx=120), 1), (dict(ldq=136), 1),
-    (dict(q=SOME + 8), 1), (dict(y=None), 2), (dict(x=None), 2), (dict(q=None), 2), (dict(ws=None), 2),
-    (dict(wsb=100), 2), (dict(m=0), 0), (dict(n=0), 0)])
+    (dict(q=SOME + 8), 1), (dict(y=None), 2), (dict(x=None), 2), (dict(q=None), 2), (dict(m=100, ws=None), 2),
+    (dict(m=100, wsb=100), 2), (dict(m=0), 0), (dict(n=0), 0)])
 def test_linear_refusals(lib, change, code):
     assert _linear(lib, **change) == code
     if code:
@@ -47,7 +47,7 @@ def test_linear_refusals(lib, change, code):
 def test_grad_and_quantizer_refusals(lib):
     assert lib.qlin_fp8_linear_grad_input(SOME, F32, 4, 100, 100, SOME, 120, 120, SOME, 1, SOME, F32, 120, SOME, 1 << 20,
                                           None) == 1
-    assert lib.qlin_fp8_linear_grad_input(SOME, F32, 4, 100, 100, SOME, 128, 128, SOME, 1, SOME, F32, 128, SOME, 16,
+    assert lib.qlin_fp8_linear_grad_input(SOME, F32, 100, 100, 100, SOME, 128, 128, SOME, 1, SOME, F32, 128, SOME, 16,
                                           None) == 2
     assert lib.qlin_fp8_linear_grad_input(SOME, F32, 4, 100, 99, SOME, 128, 128, SOME, 1, SOME, F32, 128, SOME, 1 << 20,
                                           None) == 2
