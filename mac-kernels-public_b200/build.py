@@ -6,21 +6,27 @@
 and computed shared-memory index, recorded and read back with qlin_bounds_check) as
 qlin/libqlin_checked.so, from objects in _build/checks/; select it with QLIN_LIB.
 
+qlin/_native.so, the call path of the small operators from torch tensors to the C ABI, is compiled from
+csrc/qlin_torch.cpp against the installed torch (no device code; it does not link libqlin.so).
+
 Each csrc/*.cu is compiled with nvcc for `-gencode arch=compute_100a,code=sm_100a` into
 _build/, then linked into one shared library with the CUDA runtime linked statically, so the
 library does not depend on which libcudart the host process (PyTorch) loaded.
 """
 import argparse
 import concurrent.futures as cf
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "qlin", "libqlin.so")
 OUT_CHECKED = os.path.join(HERE, "qlin", "libqlin_checked.so")
+OUT_NATIVE = os.path.join(HERE, "qlin", "_native.so")
 BUILD = os.path.join(HERE, "_build")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
@@ -46,6 +52,25 @@ def compile_one(src, verbose=False, checks=False):
     return obj, (r.stdout + r.stderr) if verbose else ""
 
 
+def build_native():
+    """qlin/_native.so: a CPython extension on torch's tensors."""
+    src = os.path.join(CSRC, "qlin_torch.cpp")
+    torch_dir = list(importlib.util.find_spec("torch").submodule_search_locations)[0]
+    deps = [src, os.path.join(HERE, "..", "include", "qlin.h"), os.path.join(torch_dir, "version.py")]
+    if os.path.exists(OUT_NATIVE) and os.path.getmtime(OUT_NATIVE) >= max(os.path.getmtime(d) for d in deps):
+        return OUT_NATIVE
+    inc, libs = os.path.join(torch_dir, "include"), os.path.join(torch_dir, "lib")
+    cuda = os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")
+    cmd = [shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared", "-I" + inc,
+           "-I" + os.path.join(inc, "torch", "csrc", "api", "include"), "-I" + cuda,
+           "-I" + sysconfig.get_paths()["include"], src, "-o", OUT_NATIVE, "-L" + libs, "-ltorch_python", "-ltorch_cpu",
+           "-lc10", "-lc10_cuda"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for {src}:\n{r.stdout}\n{r.stderr}")
+    return OUT_NATIVE
+
+
 def build(jobs=None, verbose=False, checks=False):
     out = OUT_CHECKED if checks else OUT
     os.makedirs(os.path.join(BUILD, "checks") if checks else BUILD, exist_ok=True)
@@ -63,6 +88,7 @@ def build(jobs=None, verbose=False, checks=False):
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stdout}\n{r.stderr}")
+    build_native()
     return out
 
 

@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import torch
 
+from ._fast import native
 from ._lib import QlinDecline, check, lib
 
 _DT = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
@@ -58,6 +59,10 @@ def fp8_linear(x, qdata, scale, bias=None, out_dtype=None):
     """y = x . W^T + bias for the weight W = qdata (float8_e4m3fn [N, K]) times `scale` (fp32
     [ceil(N/128), ceil(K/128)], one per block).  x [..., K] in f32, f16 or bf16, quantized per row and block of
     128 columns; K a multiple of 16.  Returns [..., N] in out_dtype (default x's)."""
+    if out_dtype is None:
+        y = native.fp8_linear(x, qdata, scale, bias)
+        if y is not None:
+            return y
     _same_device("fp8_linear", x, qdata)
     q, sc = _weight("fp8_linear", qdata, scale)
     n, k = q.shape
@@ -93,6 +98,10 @@ def fp8_linear(x, qdata, scale, bias=None, out_dtype=None):
 def fp8_linear_grad_input(dy, qdata, scale, out_dtype=None):
     """dx = dy . W for the frozen weight of fp8_linear; dy [..., N] float, quantized per row and block of 128 of
     its N columns, returns [..., K] in out_dtype (default dy's).  The weight is read as it is stored."""
+    if out_dtype is None:
+        dx = native.fp8_linear_grad_input(dy, qdata, scale)
+        if dx is not None:
+            return dx
     _same_device("fp8_linear_grad_input", dy, qdata)
     q, sc = _weight("fp8_linear_grad_input", qdata, scale)
     n, k = q.shape

@@ -15,6 +15,7 @@ import ctypes
 
 import torch
 
+from ._fast import native
 from ._lib import QlinDecline, check, lib
 
 _DT = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
@@ -26,6 +27,9 @@ def rotary_table(positions, axes_dim, theta=10000.0):
     """fp32 [..., sum(axes_dim) / 2, 2], (cos, sin) of each pair's angle: positions [..., A] (float32, int32 or
     int64) holds a coordinate per axis, axis a turns axes_dim[a] / 2 pairs, pair i of it by
     positions[..., a] * theta ** (-2 i / axes_dim[a])."""
+    out = native.rotary_table(positions, axes_dim, float(theta))
+    if out is not None:
+        return out
     if not positions.is_cuda:
         raise NotImplementedError("qlin runs on CUDA tensors only (there is no CPU path)")
     axes = len(axes_dim)
@@ -103,6 +107,10 @@ def qk_norm_rotary(q, k, q_weight, k_weight, table, eps=1e-6, interleaved=True, 
     values (2 i, 2 i + 1), or (i, i + P) where interleaved is false; values past 2 P are normed only.  `out`: two
     tensors of the inputs' shapes and dtype to write to, e.g. slices of the buffers of a joint attention (they may
     not overlap the inputs)."""
+    if out is None:
+        got = native.qk_norm_rotary(q, k, q_weight, k_weight, table, eps, interleaved)
+        if got is not None:
+            return got
     what = "qk_norm_rotary"
     q = _heads(what, "q", q)
     k = _heads(what, "k", k, q)
@@ -130,6 +138,9 @@ def qk_norm_rotary(q, k, q_weight, k_weight, table, eps=1e-6, interleaved=True, 
 def qk_norm_rotary_backward(dq, dk, q, k, q_weight, k_weight, table, eps=1e-6, interleaved=True):
     """(gradient of q, of k, of q_weight, of k_weight) for the gradients dq, dk of qk_norm_rotary's outputs; a
     weight that is None has None.  The weights' gradients are fp32 sums over all rows, in a fixed order."""
+    got = native.qk_norm_rotary_backward(dq, dk, q, k, q_weight, k_weight, table, eps, interleaved)
+    if got is not None:
+        return got
     what = "qk_norm_rotary_backward"
     q = _heads(what, "q", q)
     k = _heads(what, "k", k, q)
