@@ -39,6 +39,7 @@ struct QuantFp8Params {
 template <int DT, bool kVec>
 __global__ void __launch_bounds__(256) quant_rows_fp8_kernel(const QuantFp8Params p) {
   constexpr int kRows = 8;
+  griddep_launch();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int row_tile = blockIdx.x / p.k_tiles;
   const int b = ((blockIdx.x - row_tile * p.k_tiles) * 8 + warp) * 2 + (lane >> 4);
@@ -160,18 +161,21 @@ static int launch_fp8(const CUtensorMap& tx, const CUtensorMap& tw, const CUtens
     attr_done[dev] = true;
   }
   const int tiles = p.m_tiles * p.n_tiles;
+  const int share = CTAS == 2 ? 2 : p.splits;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(CTAS * std::min(tiles, sm_count() / CTAS));
+  cfg.gridDim = dim3((unsigned)(share * std::min(tiles, sm_count() / share)));
   cfg.blockDim = dim3(Cfg::kThreads);
   cfg.dynamicSmemBytes = Cfg::kSmem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = CTAS;
+  attr[0].val.clusterDim.x = (unsigned)share;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // set up while the quantizer runs
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = p.kb > 0 ? 2 : 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tx, tw, ty, p);
   if (e != cudaSuccess) {
     set_error("fp8 gemm launch failed: %s", cudaGetErrorString(e));
@@ -235,6 +239,31 @@ static int run_fp8_small(int x_dtype, const CUtensorMap& tw, const Fp8SmallParam
 
 // Up to this many tokens the small-M kernel runs, which quantizes them itself and needs no workspace.
 constexpr int64_t kSmallM = 64;
+
+// Which kernel and how many CTAs to a tile.  A block of 128 contraction indices takes a pair's 256 x 256 tile
+// about 800 clocks and a single CTA's 128 x 128 tile about 450 (measured at full machines), so the pair wins where
+// both fill their last wave alike.  Where the single tiles leave half of the machine free, 2, 4 or 8 CTAs share a
+// tile's contraction, at least 4 blocks each; joining their sums costs about 3 blocks' time.
+struct Fp8Plan {
+  bool pair;
+  int splits;
+};
+
+static Fp8Plan plan_fp8(int64_t m_tiles, int64_t n_tiles, int64_t kb) {
+  const int64_t sms = sm_count();
+  const auto waves = [](int64_t tiles, int64_t at_once) { return (tiles + at_once - 1) / at_once; };
+  Fp8Plan best{true, 1};
+  int64_t cost = waves(((m_tiles + 1) / 2) * ((n_tiles + 1) / 2), sms / 2) * kb * 800;
+  for (int s = 1; s <= 8; s *= 2) {
+    if (s > 1 && (m_tiles * n_tiles * s > sms || kb < 4 * s)) break;
+    const int64_t c = waves(m_tiles * n_tiles, sms / s) * ((kb + s - 1) / s + (s > 1 ? 3 : 0)) * 450;
+    if (c < cost) {
+      cost = c;
+      best = Fp8Plan{false, s};
+    }
+  }
+  return best;
+}
 
 static size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
 
@@ -345,12 +374,14 @@ static int fp8_product(const char* what, const void* x, int x_dtype, int64_t m, 
   p.lim_y = (m - 1) * ldy + out;
   p.lim_sx = (long long)kb * m;
   p.lim_sw = lim_sw;
-  const bool pair = m > 128 && out > 128;
   const int64_t m_tiles = (m + 127) / 128, n_tiles = (out + 127) / 128;
   if (m_tiles * n_tiles > 0x7fffffff) {
     set_error("%s: too many output tiles", what);
     return QLIN_EINVAL;
   }
+  const Fp8Plan plan = plan_fp8(m_tiles, n_tiles, kb);
+  const bool pair = plan.pair;
+  p.splits = plan.splits;
   p.m_tiles = (int)(pair ? (m_tiles + 1) / 2 : m_tiles);
   p.n_tiles = (int)(pair ? (n_tiles + 1) / 2 : n_tiles);
   if (p.tma_out) {

@@ -39,6 +39,7 @@ struct Fp8Params {
   void* y;
   int y_dtype;      // OutDType
   long long ldy;
+  int splits;       // single CTAs only: CTAs (a cluster) that share a tile's contraction
   int tma_out;      // y's rows are 16-byte aligned: the output leaves through tmap_y
   DeviceStatus* status;
   // Element counts of the caller's buffers for the QLIN_CHECKS build (unused otherwise).
@@ -60,6 +61,7 @@ struct Fp8Cfg {
   static constexpr uint32_t kOutWarp = 32 * kCols * 2;  // output staging of a warp: its tokens' rows, 2 bytes a value
   static constexpr int kSmem = 1024 + kStages * (int)(kAStage + kBStage) + kEpiWarps * (int)kOutWarp + 512;
   static_assert(CTAS == 1 || CTAS == 2, "one CTA or a pair");
+  static_assert(128 * 132 * 4 <= kStages * (int)(kAStage + kBStage), "the joined sums fit over the operand ring");
   static_assert(kBRows == 128, "the transposed operand is one 128-column block");
 };
 
@@ -72,6 +74,19 @@ __device__ __forceinline__ void fp8_tile(int t, int m_tiles, int n_tiles, int& m
   const int rows = min(kGroup, m_tiles - g * kGroup);
   nt = r / rows;
   mt = g * kGroup + (r - nt * rows);
+}
+
+// Pitch of a token's sums in shared memory, in floats: 16 bytes past a multiple of 128, so that the lanes of a
+// store (a token each) fall on different banks.
+constexpr int kJoinPitch = 132;
+
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
 }
 
 // (a0, a1) += s * (p0, p1)
@@ -127,8 +142,12 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
   const int lane = threadIdx.x & 31;
   const uint32_t rank = CTAS == 2 ? cluster_ctarank() : 0;
   const int num_tiles = p.m_tiles * p.n_tiles;
-  const int tile0 = blockIdx.x / CTAS;
-  const int tile_step = gridDim.x / CTAS;
+  const int share = CTAS == 2 ? 2 : p.splits;  // CTAs to a tile
+  const int tile0 = blockIdx.x / share;
+  const int tile_step = gridDim.x / share;
+  const int part_k = CTAS == 2 ? 0 : blockIdx.x % share;
+  const int b_begin = CTAS == 2 ? 0 : (int)((long long)p.kb * part_k / share);
+  const int b_end = CTAS == 2 ? p.kb : (int)((long long)p.kb * (part_k + 1) / share);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -166,6 +185,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
   if constexpr (CTAS == 2) cluster_sync();  // both CTAs' barriers are initialized before any remote arrive
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  griddep_wait();  // the quantizer's codes and scales
 
   // setmaxnreg: 2 x 224 + 56 = 3 x 168, the registers of an SM quarter's three warps at launch
   if (warp < 4) {
@@ -181,7 +201,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
           fp8_tile(t, p.m_tiles, p.n_tiles, mt, nt);
           const int m0 = (mt * CTAS + (int)rank) * 128;
           const int n0 = nt * TN + (int)rank * Cfg::kBRows;
-          for (int b = 0; b < p.kb; ++b, ++it) {
+          for (int b = b_begin; b < b_end; ++b, ++it) {
             const int s = it % STAGES;
             if (!mbar_wait(&empty[s], ((it / STAGES) & 1) ^ 1, abort_flag, p.status, 0x41)) { ok = false; break; }
             if (rank == 0) mbar_arrive_expect_tx(&full[s], CTAS * (Cfg::kAStage + Cfg::kBStage));
@@ -214,7 +234,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
         uint32_t it = 0;
         bool ok = true;
         for (int t = tile0; t < num_tiles && ok; t += tile_step) {
-          for (int b = 0; b < p.kb; ++b, ++it) {
+          for (int b = b_begin; b < b_end; ++b, ++it) {
             const int s = it % STAGES;
             const uint32_t buf = it % NB;
             if (!mbar_wait<CTAS == 2>(&full[s], (it / STAGES) & 1, abort_flag, p.status, 0x42) ||
@@ -270,7 +290,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
       const int n0 = nt * TN + part * kCols;  // kCols channels from here, inside one 128-channel block
       const long long sw_off = (long long)min(n0 / 128, (p.N - 1) / 128) * p.sw_out;
       float acc[kCols];  // the sums start from the bias
-      if (p.bias_kind != 0) {
+      if (p.bias_kind != 0 && part_k == 0) {
 #pragma unroll
         for (int c0 = 0; c0 < kCols; c0 += 32) {
           const float mine = n0 + c0 + lane < p.N ? fp8_bias(p.bias, p.bias_kind, n0 + c0 + lane, p.N) : 0.f;
@@ -284,8 +304,8 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
       // Scales come from L2, at times from HBM: a token's are asked for kAhead blocks before their use, and
       // the weight's, one for all lanes, 32 blocks at a time, a lane each.
       constexpr int kAhead = 4;
-      const float* sx_next = p.sx + min(m, p.M - 1);
-      int left = p.kb - 1;  // blocks after the one sx_next points at
+      const float* sx_next = p.sx + (long long)b_begin * p.ld_sx + min(m, p.M - 1);
+      int left = b_end - b_begin - 1;  // blocks after the one sx_next points at
       auto take_sx = [&]() {
         const float v = qchk(BS_FP8_SCALE, sx_next - p.sx, p.lim_sx) ? __ldg(sx_next) : 0.f;
         if (left > 0) sx_next += p.ld_sx;
@@ -293,17 +313,18 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
         return v;
       };
       auto take_sw = [&](int b) {
-        const long long i = sw_off + (long long)min(b + lane, p.kb - 1) * p.sw_red;
+        const long long i = sw_off + (long long)min(b_begin + b + lane, p.kb - 1) * p.sw_red;
         return qchk(BS_FP8_SCALE, i, p.lim_sw) ? __ldg(p.sw + i) : 0.f;
       };
-      float sx[kAhead], sw = p.kb > 0 ? take_sw(0) : 0.f;
+      float sx[kAhead], sw = p.kb > 0 ? take_sw(0) : 0.f;  // b counts from b_begin here
+      const int blocks = b_end - b_begin;
 #pragma unroll
       for (int u = 0; u < kAhead; ++u) sx[u] = p.kb > 0 ? take_sx() : 0.f;
-      for (int b0 = 0; b0 < p.kb && ok; b0 += kAhead) {
+      for (int b0 = 0; b0 < blocks && ok; b0 += kAhead) {
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
           const int b = b0 + u;
-          if (b >= p.kb) break;
+          if (b >= blocks) break;
           const float s = sx[u] * __shfl_sync(0xffffffffu, sw, b & 31);
           if ((b & 31) == 31) sw = take_sw(b + 1);
           sx[u] = take_sx();
@@ -335,6 +356,15 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
         }
       }
       if (!ok) break;
+      if (CTAS == 1 && share > 1) {  // this CTA's sums, for the cluster: rows of kJoinPitch floats over the operand ring
+        float* row = reinterpret_cast<float*>(sa) + r * kJoinPitch + part * kCols;
+        if (qchk_smem(BS_FP8_SMEM, smem_raw, row, kCols * 4)) {
+#pragma unroll
+          for (int j = 0; j < kCols; j += 4)
+            *reinterpret_cast<float4*>(row + j) = make_float4(acc[j], acc[j + 1], acc[j + 2], acc[j + 3]);
+        }
+        break;
+      }
       // The warp's 32 rows go through its own staging buffer, 128 bytes of each row at a time, 16-byte pieces
       // swizzled by the row; they leave as TMA stores (clipped at M and N), which the next tile's products
       // do not wait for, or, where y's rows are not 16-byte aligned, as plain stores along the rows.
@@ -412,6 +442,44 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
   // Warps 0 and 1 ran their loops on one elected lane; reconverge before the block barrier
   // (barrier.sync is .aligned) and before the warp-wide TMEM dealloc.
   __syncwarp();
+  if (CTAS == 1 && share > 1) {
+    // Every CTA of the cluster joins its share of the tile's tokens, in the order of the parts: a warp to a
+    // token, four channels to a lane.
+    const bool aborted = *abort_flag != 0;
+    cluster_sync();
+    int mt, nt;
+    fp8_tile(tile0, p.m_tiles, p.n_tiles, mt, nt);
+    const int n = nt * TN + lane * 4;
+    for (int r = part_k + share * warp; r < 128 && !aborted; r += share * (Cfg::kThreads / 32)) {
+      const int m = mt * 128 + r;
+      if (m >= p.M || n >= p.N) continue;
+      float o[4] = {};
+      for (int c = 0; c < share; ++c) {
+        const float4 v = ld_cluster_f32x4(cluster_map(reinterpret_cast<float*>(sa) + r * kJoinPitch + lane * 4, c));
+        o[0] += v.x;
+        o[1] += v.y;
+        o[2] += v.z;
+        o[3] += v.w;
+      }
+      const long long at = (long long)m * p.ldy + n;
+      if (p.tma_out && n + 4 <= p.N && qchk_span(BS_FP8_Y, at, 4, p.lim_y)) {
+        if (p.y_dtype == OUT_F32)
+          *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.y) + at) = make_float4(o[0], o[1], o[2], o[3]);
+        else
+          *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.y) + at) =
+              make_uint2(pack_out2(p.y_dtype, o[0], o[1]), pack_out2(p.y_dtype, o[2], o[3]));
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (n + j >= p.N || !qchk(BS_FP8_Y, at + j, p.lim_y)) continue;
+          if (p.y_dtype == OUT_F32) reinterpret_cast<float*>(p.y)[at + j] = o[j];
+          else if (p.y_dtype == OUT_F16) reinterpret_cast<__half*>(p.y)[at + j] = __float2half_rn(o[j]);
+          else reinterpret_cast<__nv_bfloat16*>(p.y)[at + j] = __float2bfloat16_rn(o[j]);
+        }
+      }
+    }
+    cluster_sync();  // no CTA leaves while another reads its sums
+  }
   tc_fence_before();
   __syncthreads();
   // The even CTA's MMAs (which write the odd CTA's TMEM and read its shared memory) have all

@@ -58,6 +58,29 @@ __device__ __forceinline__ void raw8_to_float(const Raw8<DT>& r, float (&f)[8]) 
   }
 }
 
+// Bit pattern, as fp32, of the largest magnitude among the 8.  Patterns of one type order like the
+// magnitudes, with the infinity and the NaNs on top, so 2-byte types are compared two at a time.
+template <int DT>
+__device__ __forceinline__ uint32_t raw8_amax_bits(const Raw8<DT>& r) {
+  const uint32_t w[4] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w};
+  if constexpr (DT == QLIN_F32) {
+    uint32_t a = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) a = max(a, w[j] & 0x7fffffffu);
+    const uint32_t x[4] = {r.v[1].x, r.v[1].y, r.v[1].z, r.v[1].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) a = max(a, x[j] & 0x7fffffffu);
+    return a;
+  } else {
+    uint32_t a = w[0] & 0x7fff7fffu;
+#pragma unroll
+    for (int j = 1; j < 4; ++j) a = __vmaxu2(a, w[j] & 0x7fff7fffu);
+    const uint32_t top = max(a >> 16, a & 0xffffu);
+    if constexpr (DT == QLIN_BF16) return top << 16;
+    return __float_as_uint(__half2float(__ushort_as_half((unsigned short)top)));
+  }
+}
+
 // 4 values times r in e4m3, the first in the low byte.
 __device__ __forceinline__ uint32_t to_e4m3x4(float a, float b, float c, float d, float r) {
   const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a * r, b * r), __NV_SATFINITE, __NV_E4M3);

@@ -44,29 +44,37 @@ struct Fp8SmallParams {
 template <int TN>
 struct Fp8SmallCfg {
   static constexpr int kThreads = 384;
-  static constexpr int kCtas = TN == 16 ? 3 : TN == 32 ? 2 : 1;  // resident on an SM
-  static constexpr int kRing = TN == 64 ? 8 : 4;  // stages, TMEM buffers and scale slots
+  static constexpr int kCtas = TN == 64 ? 1 : 2;  // resident on an SM
+  static constexpr int kRing = TN == 64 ? 8 : TN == 32 ? 5 : 6;  // stages, TMEM buffers and scale slots
   static constexpr uint32_t kWStage = 128 * 128;
   static constexpr uint32_t kXStage = TN * 128;
-  static constexpr uint32_t kTmemCols = kRing * TN;
+  static constexpr uint32_t kTmemCols = TN == 64 ? 512 : TN == 32 ? 256 : 128;  // at least kRing * TN
   static constexpr int kSmem = 1024 + kRing * (int)(kWStage + kXStage) + kRing * TN * 4 + 256;
-  static_assert(kCtas * kTmemCols <= 512 && kCtas * kSmem <= 228 * 1024, "resident CTAs");
+  static_assert(kRing * TN <= kTmemCols && kCtas * kTmemCols <= 512 && kCtas * kSmem <= 228 * 1024, "resident CTAs");
   static_assert(TN * 128 * 4 <= kRing * (int)kWStage, "the joined sums fit into the weight ring");
 };
 
-// 8 consecutive values of a row, zeros past column K.
+// 8 consecutive values of row m from column c as they are stored, zeros past M and K.  Rows that do not take
+// 16-byte loads are gathered value by value.
 template <int DT>
-__device__ __forceinline__ void small_load8(const Fp8SmallParams& p, int m, int c, float (&f)[8]) {
+__device__ __forceinline__ Raw8<DT> small_load8(const Fp8SmallParams& p, int m, int c) {
+  Raw8<DT> raw{};
   const long long at = (long long)m * p.ldx + c;
+  if (m >= p.M || c >= p.K) return raw;
   if (p.x_vec && c + 8 <= p.K) {
-    Raw8<DT> raw{};
     if (qchk_span(BS_FP8_X, at, 8, p.lim_x)) raw = load_raw8<DT>(p.x, at);
-    raw8_to_float<DT>(raw, f);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      f[j] = (c + j < p.K && qchk(BS_FP8_X, at + j, p.lim_x)) ? load_elem<DT>(p.x, at + j) : 0.f;
+    return raw;
   }
+  uint32_t w[DT == QLIN_F32 ? 8 : 4] = {};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (c + j >= p.K || !qchk(BS_FP8_X, at + j, p.lim_x)) continue;
+    if constexpr (DT == QLIN_F32) w[j] = reinterpret_cast<const uint32_t*>(p.x)[at + j];
+    else w[j / 2] |= (uint32_t) reinterpret_cast<const uint16_t*>(p.x)[at + j] << (16 * (j & 1));
+  }
+  raw.v[0] = make_uint4(w[0], w[1], w[2], w[3]);
+  if constexpr (DT == QLIN_F32) raw.v[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  return raw;
 }
 
 __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
@@ -105,7 +113,7 @@ fp8_small_kernel(const __grid_constant__ CUtensorMap tmap_w, const Fp8SmallParam
   if (threadIdx.x == 0) {
     for (int s = 0; s < R; ++s) {
       mbar_init(&w_full[s], 1);
-      mbar_init(&x_full[s], 4);
+      mbar_init(&x_full[s], 1);
       mbar_init(&empty[s], 1);
       mbar_init(&acc_full[s], 1);
       mbar_init(&acc_empty[s], 4);
@@ -179,52 +187,68 @@ fp8_small_kernel(const __grid_constant__ CUtensorMap tmap_w, const Fp8SmallParam
     }
   } else if (warp >= 4 && warp < 8) {
     // --------------------------------------------------------------------- quantizers
-    // 16 lanes to a token's block, two tokens at a time; a warp takes every fourth pair of tokens.
-    constexpr int kPairs = TN / 8;
-    const int j0 = (warp - 4) * 2 + (lane >> 4), col = (lane & 15) * 8;
-    float f[kPairs][8];
-    auto load = [&](int i) {
+    // A warp takes every fourth block, 8 tokens of it at a time, 16 lanes to a token's block; the next 8
+    // tokens' values (of this or of its next block) are in flight meanwhile.
+    constexpr int kPairs = 4;
+    const int groups = (min(p.M, TN) + 7) / 8;
+    const int col = (lane & 15) * 8;
+    Raw8<DT> raw[kPairs];
+    auto load = [&](int i, int g) {
 #pragma unroll
-      for (int u = 0; u < kPairs; ++u) {
-        const int j = j0 + u * 8;
-        if (j < p.M) small_load8<DT>(p, j, (b_begin + i) * 128 + col, f[u]);
-        else {
+      for (int u = 0; u < kPairs; ++u)
+        raw[u] = small_load8<DT>(p, g * 8 + u * 2 + (lane >> 4), (b_begin + i) * 128 + col);
+    };
+    bool ok = true;
+    if (warp - 4 < blocks) load(warp - 4, 0);
+    for (int i = warp - 4; i < blocks && ok; i += 4) {
+      const int s = i % R;
+      uint8_t* tile = sx + s * Cfg::kXStage;
+      for (int g = 0; g < groups; ++g) {
+        Raw8<DT> now[kPairs];  // kept as stored: as fp32 they would take twice the registers
+        uint32_t a[kPairs];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) f[u][e] = 0.f;
+        for (int u = 0; u < kPairs; ++u) {
+          now[u] = raw[u];
+          a[u] = max(kAmaxFloorBits, raw8_amax_bits<DT>(now[u]));
+        }
+        if (g + 1 < groups) load(i, g + 1);
+        else if (i + 4 < blocks) load(i + 4, 0);
+        // each lane ends up with the maximum of pair (lane >> 2) & 3 of its half, as in the row quantizer
+#pragma unroll
+        for (int o = 8, n = 2; o > 2; o >>= 1, n >>= 1) {
+          const bool up = lane & o;
+#pragma unroll
+          for (int u = 0; u < n; ++u) {
+            const uint32_t give = up ? a[u] : a[u + n], keep = up ? a[u + n] : a[u];
+            a[u] = max(keep, __shfl_xor_sync(0xffffffffu, give, o));
+          }
+        }
+        a[0] = max(a[0], __shfl_xor_sync(0xffffffffu, a[0], 2));
+        a[0] = max(a[0], __shfl_xor_sync(0xffffffffu, a[0], 1));
+        const float amax = __uint_as_float(a[0]);
+        const float up = __fdiv_rn(kE4m3Max, amax);
+        if (g == 0) {
+          const uint32_t ph = ((i / R) & 1) ^ 1;
+          if (!mbar_wait(&empty[s], ph, abort_flag, p.status, 0x55) ||
+              !mbar_wait(&acc_empty[s], ph, abort_flag, p.status, 0x56)) {
+            ok = false;
+            break;
+          }
+        }
+        if ((lane & 3) == 0) scale[s * TN + g * 8 + ((lane >> 2) & 3) * 2 + (lane >> 4)] = __fdiv_rn(amax, kE4m3Max);
+#pragma unroll
+        for (int u = 0; u < kPairs; ++u) {
+          const float r = __shfl_sync(0xffffffffu, up, (lane & 16) | (u << 2));
+          const int j = g * 8 + u * 2 + (lane >> 4);
+          float f[8];
+          raw8_to_float<DT>(now[u], f);
+          uint8_t* at = tile + j * 128 + ((((lane & 15) >> 1) ^ (j & 7)) << 4) + (lane & 1) * 8;
+          if (qchk_smem(BS_FP8_SMEM, smem_raw, at, 8))
+            *reinterpret_cast<uint2*>(at) = make_uint2(to_e4m3x4(f[0], f[1], f[2], f[3], r),
+                                                       to_e4m3x4(f[4], f[5], f[6], f[7], r));
         }
       }
-    };
-    if (blocks > 0) load(0);
-    for (int i = 0; i < blocks; ++i) {
-      const int s = i % R;
-      uint2 q[kPairs];
-      float mine[kPairs];
-#pragma unroll
-      for (int u = 0; u < kPairs; ++u) {
-        uint32_t a = kAmaxFloorBits;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) a = max(a, __float_as_uint(f[u][e]) & 0x7fffffffu);
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
-        const float amax = __uint_as_float(a);
-        const float r = __fdiv_rn(kE4m3Max, amax);
-        mine[u] = __fdiv_rn(amax, kE4m3Max);
-        q[u] = make_uint2(to_e4m3x4(f[u][0], f[u][1], f[u][2], f[u][3], r),
-                          to_e4m3x4(f[u][4], f[u][5], f[u][6], f[u][7], r));
-      }
-      if (i + 1 < blocks) load(i + 1);  // in flight while the ring slot is awaited
-      const uint32_t ph = ((i / R) & 1) ^ 1;
-      if (!mbar_wait(&empty[s], ph, abort_flag, p.status, 0x55) ||
-          !mbar_wait(&acc_empty[s], ph, abort_flag, p.status, 0x56))
-        break;
-      uint8_t* tile = sx + s * Cfg::kXStage;
-#pragma unroll
-      for (int u = 0; u < kPairs; ++u) {
-        const int j = j0 + u * 8;
-        uint8_t* at = tile + j * 128 + ((((lane & 15) >> 1) ^ (j & 7)) << 4) + (lane & 1) * 8;
-        if (qchk_smem(BS_FP8_SMEM, smem_raw, at, 8)) *reinterpret_cast<uint2*>(at) = q[u];
-        if ((lane & 15) == 0) scale[s * TN + j] = mine[u];
-      }
+      if (!ok) break;
       fence_proxy_async_smem();  // the MMA reads the tile through the async proxy
       __syncwarp();
       if (lane == 0) mbar_arrive(&x_full[s]);

@@ -219,6 +219,10 @@ __device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wa
 __device__ __forceinline__ void fence_proxy_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
+// Programmatic dependent launch: the next kernel on the stream, if it was launched for it, may be set up from
+// here on; and a kernel so launched waits until the one before it has completed.  Without it, both do nothing.
+__device__ __forceinline__ void griddep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // Registers of a thread from here on, for whole warpgroups; an increase waits until others released them.
 template <int N>
 __device__ __forceinline__ void setmaxnreg_inc() {
