@@ -83,8 +83,11 @@ template <int CAP, typename POS>
 __global__ void __launch_bounds__(256) rotary_table_kernel(const __grid_constant__ RotTableParams<CAP> p) {
   const int pair = blockIdx.y * 32 + threadIdx.x;
   if (pair >= p.pairs) return;
-  const unsigned long long turn = p.turn[pair];
-  const int axis = p.axis[pair];
+  // Read by address, as ordinary memory: the constant cache serves one lane's entry at a time.
+  const RotTableParams<CAP>* params = &p;
+  asm volatile("" : "+l"(params));
+  const unsigned long long turn = params->turn[pair];
+  const int axis = params->axis[pair];
   const POS* pos = reinterpret_cast<const POS*>(p.pos);
   constexpr int kTokens = 4;
   const long long step = (long long)gridDim.x * 8;
@@ -286,6 +289,34 @@ __device__ __forceinline__ void load_turn(const HeadParams& p, long long token_r
   }
 }
 
+// The lane's 8 values of the weight; its two pieces start on multiples of 4 values (the vector kernels take
+// weights whose address is a multiple of 4 values too).
+template <class Plan>
+__device__ __forceinline__ void load_weight(const void* w, int dt, const Plan& plan, int D, float (&f)[8]) {
+  if (w == nullptr || !plan.on || !qchk_span(BS_ROT_IN, plan.o0, 4, D) || !qchk_span(BS_ROT_IN, plan.o1, 4, D)) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = plan.on ? 1.f : 0.f;
+  } else if (dt == QLIN_F32) {
+    pieces_to_float<QLIN_F32>(load_pieces<QLIN_F32, false>(w, 0, plan.o0, plan.o1), f);
+  } else if (dt == QLIN_F16) {
+    pieces_to_float<QLIN_F16>(load_pieces<QLIN_F16, false>(w, 0, plan.o0, plan.o1), f);
+  } else {
+    pieces_to_float<QLIN_BF16>(load_pieces<QLIN_BF16, false>(w, 0, plan.o0, plan.o1), f);
+  }
+}
+
+// Batch and position of a token.
+__device__ __forceinline__ void token_of(const HeadParams& p, long long token, long long& b, long long& l) {
+  if (p.tokens <= 0x7fffffff) {
+    const uint32_t q = (uint32_t)token / (uint32_t)p.L;
+    b = q;
+    l = (uint32_t)token - q * (uint32_t)p.L;
+  } else {
+    b = token / p.L;
+    l = token - b * p.L;
+  }
+}
+
 template <int G>
 __device__ __forceinline__ float group_sum(float v) {
 #pragma unroll
@@ -293,32 +324,30 @@ __device__ __forceinline__ float group_sum(float v) {
   return v;
 }
 
-// Forward.  A row is G lanes of 8 values; a warp takes one token's q or k heads (or a share of them, where
-// there are few tokens), 32 / G rows at a time with kUnroll loads in flight, and keeps the token's cosines
-// and sines and the weight in registers.
+// Forward.  A row is G lanes of 8 values; a warp takes a share of a token's q or k heads (all of them where
+// there are tokens enough), 32 / G rows at a time with kUnroll loads in flight, and keeps the token's cosines
+// and sines in registers, and the weight for all of its tokens.  blockIdx.y is the share.
 template <int DT, int G, bool kInter>
-__global__ void __launch_bounds__(256) qk_norm_rotary_kernel(const __grid_constant__ HeadParams p) {
+__global__ void __launch_bounds__(256, 4) qk_norm_rotary_kernel(const __grid_constant__ HeadParams p) {
   constexpr int R = 32 / G;
-  constexpr int kUnroll = 4;
+  constexpr int kUnroll = DT == QLIN_F32 ? 2 : 4;
   const int lane = threadIdx.x & 31;
-  const long long item = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int per = p.side[0].chunks + p.side[1].chunks;
-  const long long token = item / per;
-  if (token >= p.tokens) return;
-  int chunk = (int)(item - token * per);
+  int chunk = blockIdx.y;
   const int which = chunk >= p.side[0].chunks ? 1 : 0;
   if (which) chunk -= p.side[0].chunks;
   const HeadSide& sd = p.side[which];
-  const long long b = token / p.L, l = token - b * p.L;
   const LanePlan<G> plan(lane, p.D, p.pairs, kInter);
+  const float inv_d = 1.f / (float)p.D;
+  const int h_begin = chunk * p.heads_per_warp, h_end = min(sd.heads, h_begin + p.heads_per_warp);
+  const long long token = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (token >= p.tokens) return;
+  long long b, l;
+  token_of(p, token, b, l);
   float c[4], s[4], w[8];
   load_turn(p, b * p.table_b + l * p.pairs, plan.pair0, c, s);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) w[j] = plan.on ? weight_at(sd.w, p.w_dtype, (j < 4 ? plan.o0 : plan.o1 - 4) + j, p.D) : 0.f;
-  const float inv_d = 1.f / (float)p.D;
+  load_weight(sd.w, p.w_dtype, plan, p.D, w);
   const long long xr = b * sd.x_b + l * sd.x_l, yr = b * sd.y_b + l * sd.y_l;
-  const int h_end = min(sd.heads, (chunk + 1) * p.heads_per_warp);
-  for (int h0 = chunk * p.heads_per_warp; h0 < h_end; h0 += R * kUnroll) {
+  for (int h0 = h_begin; h0 < h_end; h0 += R * kUnroll) {
     Pieces<DT> raw[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
@@ -331,6 +360,7 @@ __global__ void __launch_bounds__(256) qk_norm_rotary_kernel(const __grid_consta
     }
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
+      if (h0 + u * R >= h_end) break;
       const int h = h0 + u * R + lane / G;
       float f[8], ss = 0.f;
       pieces_to_float<DT>(raw[u], f);
@@ -351,34 +381,35 @@ __global__ void __launch_bounds__(256) qk_norm_rotary_kernel(const __grid_consta
 // Backward.  The CTAs of a side walk over its (token, share of heads) items; every lane sums its 8 columns'
 // g * xhat in fp32, the CTA joins its rows in a fixed order and leaves one partial row of dw, and the
 // kernel below adds those up, also in a fixed order.
+constexpr int kBwdCtas = 2;  // resident on an SM: 128 registers a thread
 template <int DT, int G, bool kInter>
-__global__ void __launch_bounds__(256) qk_norm_rotary_bwd_kernel(const __grid_constant__ HeadParams p) {
+__global__ void __launch_bounds__(256, kBwdCtas) qk_norm_rotary_bwd_kernel(const __grid_constant__ HeadParams p) {
   constexpr int R = 32 / G;
-  constexpr int kUnroll = 2;
+  constexpr int kUnroll = DT == QLIN_F32 ? 2 : 3;
   __shared__ float part[8 * R][G * 8];
+  griddep_launch();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int which = blockIdx.x >= (unsigned)p.ctas[0] ? 1 : 0;
   const int cta = which ? blockIdx.x - p.ctas[0] : blockIdx.x;
   const HeadSide& sd = p.side[which];
   const LanePlan<G> plan(lane, p.D, p.pairs, kInter);
   float w[8], dw[8];
+  load_weight(sd.w, p.w_dtype, plan, p.D, w);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    w[j] = plan.on ? weight_at(sd.w, p.w_dtype, (j < 4 ? plan.o0 : plan.o1 - 4) + j, p.D) : 0.f;
-    dw[j] = 0.f;
-  }
+  for (int j = 0; j < 8; ++j) dw[j] = 0.f;
   const float inv_d = 1.f / (float)p.D;
   const long long items = p.tokens * sd.chunks;
   for (long long item = (long long)cta * 8 + warp; item < items; item += (long long)p.ctas[which] * 8) {
-    const long long token = item / sd.chunks;
+    const long long token = sd.chunks == 1 ? item : item / sd.chunks;
     const int chunk = (int)(item - token * sd.chunks);
-    const long long b = token / p.L, l = token - b * p.L;
+    long long b, l;
+    token_of(p, token, b, l);
     float c[4], s[4];
     load_turn(p, b * p.table_b + l * p.pairs, plan.pair0, c, s);
     const long long xr = b * sd.x_b + l * sd.x_l, yr = b * sd.y_b + l * sd.y_l, gr = b * sd.dy_b + l * sd.dy_l;
     const int h_end = min(sd.heads, (chunk + 1) * p.heads_per_warp);
-    for (int h0 = chunk * p.heads_per_warp; h0 < h_end; h0 += R * kUnroll) {
-      Pieces<DT> rx[kUnroll], rg[kUnroll];
+    Pieces<DT> rx[kUnroll], rg[kUnroll];
+    auto load = [&](int h0) {
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) {
         const int h = h0 + u * R + lane / G;
@@ -392,12 +423,23 @@ __global__ void __launch_bounds__(256) qk_norm_rotary_bwd_kernel(const __grid_co
           rg[u] = load_pieces<DT, kInter>(sd.dy, grow, plan.o0, plan.o1);
         }
       }
+    };
+    const int h_begin = chunk * p.heads_per_warp;
+    load(h_begin);
+    for (int h0 = h_begin; h0 < h_end; h0 += R * kUnroll) {
+      Pieces<DT> cx[kUnroll], cg[kUnroll];  // the next rows' loads are in flight during these rows' arithmetic
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        cx[u] = rx[u];
+        cg[u] = rg[u];
+      }
+      if (h0 + R * kUnroll < h_end) load(h0 + R * kUnroll);
 #pragma unroll
       for (int u = 0; u < kUnroll; ++u) {
         const int h = h0 + u * R + lane / G;
         float x[8], g[8], ss = 0.f, dot = 0.f;
-        pieces_to_float<DT>(rx[u], x);
-        pieces_to_float<DT>(rg[u], g);
+        pieces_to_float<DT>(cx[u], x);
+        pieces_to_float<DT>(cg[u], g);
         rotate4<kInter, true>(g, c, s);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -447,6 +489,7 @@ struct DwParams {
 // dw = the sum of the partial rows: 32 columns to a CTA, 32 rows at a time, one rounding to the weight's type.
 __global__ void __launch_bounds__(1024) dw_sum_kernel(const DwParams p) {
   __shared__ float part[32][33];
+  griddep_wait();
   const int which = blockIdx.y;
   const int i = blockIdx.x * 32 + threadIdx.x;
   if (p.out[which] == nullptr) return;
@@ -474,6 +517,7 @@ __global__ void __launch_bounds__(1024) dw_sum_kernel(const DwParams p) {
 template <int DT, bool kBack>
 __global__ void __launch_bounds__(256) qk_norm_rotary_any_kernel(const __grid_constant__ HeadParams p) {
   extern __shared__ float warp_dw[];  // backward: [8][D]
+  if constexpr (kBack) griddep_launch();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int which = blockIdx.x >= (unsigned)p.ctas[0] ? 1 : 0;
   const int cta = which ? blockIdx.x - p.ctas[0] : blockIdx.x;
@@ -616,7 +660,7 @@ static int lanes_per_row(int D) {
 // Backward: the CTAs of both sides together, each with a partial row of dw.  Four resident CTAs on each SM
 // or fewer where there are fewer rows.
 static void plan_bwd(long long tokens, int hq, int hk, int rows_per_cta, int (&ctas)[2]) {
-  const long long most = 4ll * sm_count();
+  const long long most = (long long)kBwdCtas * sm_count();
   const long long rows = tokens * (hq + hk);
   const long long want = std::max<long long>(2, std::min<long long>(most, rows / rows_per_cta));
   const int heads[2] = {hq, hk};
@@ -625,7 +669,7 @@ static void plan_bwd(long long tokens, int hq, int hk, int rows_per_cta, int (&c
 }
 
 template <int DT, bool kInter>
-static void launch_rows(const HeadParams& p, int g, bool back, unsigned grid, cudaStream_t s) {
+static void launch_rows(const HeadParams& p, int g, bool back, dim3 grid, cudaStream_t s) {
   switch (g) {
 #define QLIN_ROWS(G)                                                                    \
   case G:                                                                               \
@@ -641,7 +685,7 @@ static void launch_rows(const HeadParams& p, int g, bool back, unsigned grid, cu
 }
 
 template <int DT>
-static void launch_dtype(const HeadParams& p, bool vec, bool back, unsigned grid, cudaStream_t s) {
+static void launch_dtype(const HeadParams& p, bool vec, bool back, dim3 grid, cudaStream_t s) {
   if (!vec) {
     if (back) qk_norm_rotary_any_kernel<DT, true><<<grid, 256, (size_t)8 * p.D * 4, s>>>(p);
     else qk_norm_rotary_any_kernel<DT, false><<<grid, 256, 0, s>>>(p);
@@ -731,6 +775,7 @@ static int head_norm(const HeadCall& a, int dtype, int64_t batch, int64_t tokens
     sd.dy = gs[i];
     sd.y = os[i];
     sd.w = ws[i];
+    vec = vec && reinterpret_cast<uintptr_t>(sd.w) % (w_dtype == QLIN_F32 ? 16 : 8) == 0;
     sd.x_b = xst[i][0]; sd.x_l = xst[i][1]; sd.x_h = xst[i][2];
     sd.y_b = ost[i][0]; sd.y_l = ost[i][1]; sd.y_h = ost[i][2];
     sd.lim_x = reach(batch, sd.x_b, tokens, sd.x_l, heads[i], sd.x_h, dim);
@@ -745,14 +790,15 @@ static int head_norm(const HeadCall& a, int dtype, int64_t batch, int64_t tokens
   }
   // A warp's share of a token's heads: all of q or of k where there are tokens enough to fill the machine
   // (about 32 warps on each SM), else as few as one set of unrolled rows.
-  const int step = std::max(1, 32 / lanes_per_row(dim)) * (a.back ? 2 : 4);
+  const int step = std::max(1, 32 / lanes_per_row(dim)) * 2;
   int per_warp = std::max(hq, hk);
   const long long warps = 32ll * sm_count();
-  while (per_warp > step && rows * ((hq + per_warp - 1) / per_warp + (hk + per_warp - 1) / per_warp) < warps)
+  const int fewest = (std::max(hq, hk) + 16383) / 16384;  // the shares are a grid dimension
+  while (per_warp > step && per_warp > 2 * fewest && rows * ((hq + per_warp - 1) / per_warp + (hk + per_warp - 1) / per_warp) < warps)
     per_warp = std::max(step, (per_warp + 1) / 2);
   p.heads_per_warp = per_warp;
   for (int i = 0; i < 2; ++i) p.side[i].chunks = (heads[i] + per_warp - 1) / per_warp;
-  unsigned grid = 0;
+  dim3 grid(1);
   if (a.back) {
     const size_t need = bwd_workspace(rows, hq, hk, dim);
     if (workspace == nullptr || workspace_bytes < need) {
@@ -762,18 +808,17 @@ static int head_norm(const HeadCall& a, int dtype, int64_t batch, int64_t tokens
     plan_bwd(rows, hq, hk, kBwdRowsPerCta, p.ctas);
     if (a.dqw != nullptr) p.side[0].dw = reinterpret_cast<float*>(workspace);
     if (a.dkw != nullptr) p.side[1].dw = reinterpret_cast<float*>(workspace) + (size_t)p.ctas[0] * dim;
-    grid = (unsigned)(p.ctas[0] + p.ctas[1]);
+    grid = dim3((unsigned)(p.ctas[0] + p.ctas[1]));
   } else if (vec) {
-    const long long items = rows * (p.side[0].chunks + p.side[1].chunks);
-    if ((items + 7) / 8 > 0x7fffffff) {
-      set_error("%s: too many rows", a.what);
+    if ((rows + 7) / 8 > 0x7fffffff) {
+      set_error("%s: too many tokens", a.what);
       return QLIN_EINVAL;
     }
-    grid = (unsigned)((items + 7) / 8);
+    grid = dim3((unsigned)((rows + 7) / 8), (unsigned)(p.side[0].chunks + p.side[1].chunks));
   } else {
     for (int i = 0; i < 2; ++i)
       p.ctas[i] = (int)std::min<long long>(8ll * sm_count(), (rows * heads[i] + 7) / 8);
-    grid = (unsigned)(p.ctas[0] + p.ctas[1]);
+    grid = dim3((unsigned)(p.ctas[0] + p.ctas[1]));
   }
   if (dtype == QLIN_F16) launch_dtype<QLIN_F16>(p, vec, a.back, grid, stream);
   else if (dtype == QLIN_BF16) launch_dtype<QLIN_BF16>(p, vec, a.back, grid, stream);
@@ -789,8 +834,17 @@ static int head_norm(const HeadCall& a, int dtype, int64_t batch, int64_t tokens
   d.out[1] = a.dkw;
   d.D = dim;
   d.w_dtype = w_dtype;
-  dw_sum_kernel<<<dim3((dim + 31) / 32, 2), dim3(32, 32), 0, stream>>>(d);
-  return rot_launched(a.what);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((dim + 31) / 32, 2);
+  cfg.blockDim = dim3(32, 32);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // set up while the rows are summed
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, dw_sum_kernel, d) != cudaSuccess) return rot_launched(a.what);
+  return QLIN_OK;
 }
 
 // This translation unit's bounds record (QLIN_CHECKS build).
