@@ -47,12 +47,14 @@ __global__ void __launch_bounds__(256) quant_rows_fp8_kernel(const QuantFp8Param
   const int c = b * 128 + (lane & 15) * 8;
   const int rows = min(kRows, p.M - m0);
   float f[kRows][8];
-  if (kVec && c + 8 <= p.K) {
+  if (c + 8 <= p.K) {
     Raw8<DT> raw[kRows];
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
       const long long at = (long long)(m0 + min(i, rows - 1)) * p.ldx + c;
-      if (qchk_span(BS_FP8_QUANT, at, 8, p.lim_x)) raw[i] = load_raw8<DT>(p.x, at);
+      raw[i] = Raw8<DT>{};
+      if (qchk_span(BS_FP8_QUANT, at, 8, p.lim_x))
+        raw[i] = kVec ? load_raw8<DT>(p.x, at) : load_raw8_any<DT>(p.x, at, p.lim_x);
     }
 #pragma unroll
     for (int i = 0; i < kRows; ++i) raw8_to_float<DT>(raw[i], f[i]);
@@ -184,10 +186,10 @@ static int launch_fp8(const CUtensorMap& tx, const CUtensorMap& tw, const CUtens
   return QLIN_OK;
 }
 
-template <int TN, bool kTrans, int DT>
+template <bool kTrans, int DT>
 static int launch_fp8_small(const CUtensorMap& tw, const Fp8SmallParams& p, cudaStream_t stream) {
-  using Cfg = Fp8SmallCfg<TN>;
-  auto kern = fp8_small_kernel<TN, kTrans, DT>;
+  using Cfg = Fp8SmallCfg;
+  auto kern = fp8_small_kernel<kTrans, DT>;
   static bool attr_done[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -223,27 +225,22 @@ static int launch_fp8_small(const CUtensorMap& tw, const Fp8SmallParams& p, cuda
   return QLIN_OK;
 }
 
-template <int TN, bool kTrans>
-static int small_of_dtype(int x_dtype, const CUtensorMap& tw, const Fp8SmallParams& p, cudaStream_t stream) {
-  if (x_dtype == QLIN_F16) return launch_fp8_small<TN, kTrans, QLIN_F16>(tw, p, stream);
-  if (x_dtype == QLIN_BF16) return launch_fp8_small<TN, kTrans, QLIN_BF16>(tw, p, stream);
-  return launch_fp8_small<TN, kTrans, QLIN_F32>(tw, p, stream);
-}
-
 template <bool kTrans>
 static int run_fp8_small(int x_dtype, const CUtensorMap& tw, const Fp8SmallParams& p, cudaStream_t stream) {
-  if (p.M <= 16) return small_of_dtype<16, kTrans>(x_dtype, tw, p, stream);
-  if (p.M <= 32) return small_of_dtype<32, kTrans>(x_dtype, tw, p, stream);
-  return small_of_dtype<64, kTrans>(x_dtype, tw, p, stream);
+  if (x_dtype == QLIN_F16) return launch_fp8_small<kTrans, QLIN_F16>(tw, p, stream);
+  if (x_dtype == QLIN_BF16) return launch_fp8_small<kTrans, QLIN_BF16>(tw, p, stream);
+  return launch_fp8_small<kTrans, QLIN_F32>(tw, p, stream);
 }
 
 // Up to this many tokens the small-M kernel runs, which quantizes them itself and needs no workspace.
-constexpr int64_t kSmallM = 64;
+constexpr int64_t kSmallM = Fp8SmallCfg::TN;
 
-// Which kernel and how many CTAs to a tile.  A block of 128 contraction indices takes a pair's 256 x 256 tile
-// about 800 clocks and a single CTA's 128 x 128 tile about 450 (measured at full machines), so the pair wins where
-// both fill their last wave alike.  Where the single tiles leave half of the machine free, 2, 4 or 8 CTAs share a
-// tile's contraction, at least 4 blocks each; joining their sums costs about 3 blocks' time.
+// Which kernel and how many CTAs to a tile.  Measured with warm operands, a block of 128 contraction indices takes
+// a pair's 256 x 256 tile about 790 clocks and a single CTA's 128 x 128 tile about 560, so the pair wins where
+// both fill their last wave alike (1024 x 4096 x 4096: 22 us against two waves of single tiles), the single tiles
+// where the pair's leave SMs idle (333 x 4096 x 5120: 14.8 us, the pair 21.9).  Where they leave half of the
+// machine free, 2, 4 or 8 CTAs share a tile's contraction, at least 4 blocks each; their join costs about 5500
+// clocks (128 x 4096 x 5120: 12.8 us shared by two, 17 alone; 128 x 1024 x 5120: 10 and 8).
 struct Fp8Plan {
   bool pair;
   int splits;
@@ -253,10 +250,10 @@ static Fp8Plan plan_fp8(int64_t m_tiles, int64_t n_tiles, int64_t kb) {
   const int64_t sms = sm_count();
   const auto waves = [](int64_t tiles, int64_t at_once) { return (tiles + at_once - 1) / at_once; };
   Fp8Plan best{true, 1};
-  int64_t cost = waves(((m_tiles + 1) / 2) * ((n_tiles + 1) / 2), sms / 2) * kb * 800;
+  int64_t cost = waves(((m_tiles + 1) / 2) * ((n_tiles + 1) / 2), sms / 2) * kb * 790;
   for (int s = 1; s <= 8; s *= 2) {
     if (s > 1 && (m_tiles * n_tiles * s > sms || kb < 4 * s)) break;
-    const int64_t c = waves(m_tiles * n_tiles, sms / s) * ((kb + s - 1) / s + (s > 1 ? 3 : 0)) * 450;
+    const int64_t c = waves(m_tiles * n_tiles, sms / s) * ((kb + s - 1) / s) * 560 + (s > 1 ? 5500 : 0);
     if (c < cost) {
       cost = c;
       best = Fp8Plan{false, s};

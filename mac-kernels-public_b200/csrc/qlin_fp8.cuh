@@ -271,6 +271,11 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
         }
       }
     }
+    if (CTAS == 1 && share > 1) {  // the two cluster barriers around the join
+      __syncwarp();
+      cluster_sync();
+      cluster_sync();
+    }
   } else {
     setmaxnreg_inc<224>();
     // --------------------------------------------------------------------- rescale + epilogue
@@ -413,6 +418,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
         } else {
           __syncwarp();
           const int rows = min(32, p.M - m_warp);
+#pragma unroll 4
           for (int rr = 0; rr < rows; ++rr) {
 #pragma unroll
             for (int q = 0; q < kN / 32; ++q) {
@@ -437,49 +443,64 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
       }
     }
     if (lane == 0) bulk_wait_all();
+    if (CTAS == 1 && share > 1) {
+      // Every CTA of the cluster joins its share of the tile's tokens, in the order of the parts: four channels
+      // to a thread, two tokens at a time, with all of their loads in flight.
+      cluster_sync();
+      const bool aborted = *abort_flag != 0;
+      int mt, nt;
+      fp8_tile(tile0, p.m_tiles, p.n_tiles, mt, nt);
+      const int n = nt * TN + lane * 4;
+      const int valid = min(128, p.M - mt * 128);
+      constexpr int kWarps = Cfg::kEpiWarps;
+      const uint32_t mine = smem_u32(reinterpret_cast<float*>(sa) + lane * 4);
+      for (int r0 = part_k + share * (warp - 4); r0 < valid && n < p.N && !aborted; r0 += share * kWarps * 2) {
+        float4 v[2][8];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int r = r0 + u * share * kWarps;
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            if (c < share && r < valid) v[u][c] = ld_cluster_f32x4(cluster_map_addr(mine + r * (kJoinPitch * 4), c));
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int r = r0 + u * share * kWarps;
+          if (r >= valid) break;
+          float o[4] = {};
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            if (c >= share) break;
+            o[0] += v[u][c].x;
+            o[1] += v[u][c].y;
+            o[2] += v[u][c].z;
+            o[3] += v[u][c].w;
+          }
+          const long long at = (long long)(mt * 128 + r) * p.ldy + n;
+          if (p.tma_out && n + 4 <= p.N && qchk_span(BS_FP8_Y, at, 4, p.lim_y)) {
+            if (p.y_dtype == OUT_F32)
+              *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.y) + at) = make_float4(o[0], o[1], o[2], o[3]);
+            else
+              *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.y) + at) =
+                  make_uint2(pack_out2(p.y_dtype, o[0], o[1]), pack_out2(p.y_dtype, o[2], o[3]));
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if (n + j >= p.N || !qchk(BS_FP8_Y, at + j, p.lim_y)) continue;
+              if (p.y_dtype == OUT_F32) reinterpret_cast<float*>(p.y)[at + j] = o[j];
+              else if (p.y_dtype == OUT_F16) reinterpret_cast<__half*>(p.y)[at + j] = __float2half_rn(o[j]);
+              else reinterpret_cast<__nv_bfloat16*>(p.y)[at + j] = __float2bfloat16_rn(o[j]);
+            }
+          }
+        }
+      }
+      cluster_sync();  // no CTA leaves while another reads its sums
+    }
   }
 
   // Warps 0 and 1 ran their loops on one elected lane; reconverge before the block barrier
   // (barrier.sync is .aligned) and before the warp-wide TMEM dealloc.
   __syncwarp();
-  if (CTAS == 1 && share > 1) {
-    // Every CTA of the cluster joins its share of the tile's tokens, in the order of the parts: a warp to a
-    // token, four channels to a lane.
-    const bool aborted = *abort_flag != 0;
-    cluster_sync();
-    int mt, nt;
-    fp8_tile(tile0, p.m_tiles, p.n_tiles, mt, nt);
-    const int n = nt * TN + lane * 4;
-    for (int r = part_k + share * warp; r < 128 && !aborted; r += share * (Cfg::kThreads / 32)) {
-      const int m = mt * 128 + r;
-      if (m >= p.M || n >= p.N) continue;
-      float o[4] = {};
-      for (int c = 0; c < share; ++c) {
-        const float4 v = ld_cluster_f32x4(cluster_map(reinterpret_cast<float*>(sa) + r * kJoinPitch + lane * 4, c));
-        o[0] += v.x;
-        o[1] += v.y;
-        o[2] += v.z;
-        o[3] += v.w;
-      }
-      const long long at = (long long)m * p.ldy + n;
-      if (p.tma_out && n + 4 <= p.N && qchk_span(BS_FP8_Y, at, 4, p.lim_y)) {
-        if (p.y_dtype == OUT_F32)
-          *reinterpret_cast<float4*>(reinterpret_cast<float*>(p.y) + at) = make_float4(o[0], o[1], o[2], o[3]);
-        else
-          *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(p.y) + at) =
-              make_uint2(pack_out2(p.y_dtype, o[0], o[1]), pack_out2(p.y_dtype, o[2], o[3]));
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (n + j >= p.N || !qchk(BS_FP8_Y, at + j, p.lim_y)) continue;
-          if (p.y_dtype == OUT_F32) reinterpret_cast<float*>(p.y)[at + j] = o[j];
-          else if (p.y_dtype == OUT_F16) reinterpret_cast<__half*>(p.y)[at + j] = __float2half_rn(o[j]);
-          else reinterpret_cast<__nv_bfloat16*>(p.y)[at + j] = __float2bfloat16_rn(o[j]);
-        }
-      }
-    }
-    cluster_sync();  // no CTA leaves while another reads its sums
-  }
   tc_fence_before();
   __syncthreads();
   // The even CTA's MMAs (which write the odd CTA's TMEM and read its shared memory) have all

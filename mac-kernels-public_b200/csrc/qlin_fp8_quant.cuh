@@ -34,6 +34,47 @@ __device__ __forceinline__ Raw8<DT> load_raw8(const void* x, long long i) {
   return r;
 }
 
+// The same from any address of the type's alignment: the aligned 16-byte words around the values, shifted.
+// `lim` is the number of values from x on that are the caller's; where the words reach past them, value by value.
+template <int DT>
+__device__ __forceinline__ Raw8<DT> load_raw8_any(const void* x, long long i, long long lim) {
+  constexpr int kBytes = DT == QLIN_F32 ? 4 : 2;
+  constexpr int kWords = DT == QLIN_F32 ? 12 : 8;  // 32-bit words read
+  constexpr int kOut = DT == QLIN_F32 ? 8 : 4;
+  const uintptr_t at = reinterpret_cast<uintptr_t>(x) + i * kBytes;
+  const uintptr_t from = at & ~uintptr_t(15);
+  uint32_t o[kOut] = {};
+  if (from >= reinterpret_cast<uintptr_t>(x) && from + kWords * 4 <= reinterpret_cast<uintptr_t>(x) + lim * kBytes) {
+    uint32_t w[kWords + 1];
+#pragma unroll
+    for (int j = 0; j < kWords / 4; ++j) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(from) + j);
+      w[4 * j] = v.x;
+      w[4 * j + 1] = v.y;
+      w[4 * j + 2] = v.z;
+      w[4 * j + 3] = v.w;
+    }
+    w[kWords] = 0;
+    const uint32_t off = (uint32_t)(at & 15);
+#pragma unroll
+    for (int j = 0; j + 2 <= kWords; ++j) w[j] = (off & 8) ? w[j + 2] : w[j];
+#pragma unroll
+    for (int j = 0; j + 1 <= kWords; ++j) w[j] = (off & 4) ? w[j + 1] : w[j];
+#pragma unroll
+    for (int j = 0; j < kOut; ++j) o[j] = kBytes == 2 ? __funnelshift_r(w[j], w[j + 1], (off & 2) * 8) : w[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if constexpr (DT == QLIN_F32) o[j] = reinterpret_cast<const uint32_t*>(x)[i + j];
+      else o[j / 2] |= (uint32_t) reinterpret_cast<const uint16_t*>(x)[i + j] << (16 * (j & 1));
+    }
+  }
+  Raw8<DT> r;
+  r.v[0] = make_uint4(o[0], o[1], o[2], o[3]);
+  if constexpr (DT == QLIN_F32) r.v[1] = make_uint4(o[4], o[5], o[6], o[7]);
+  return r;
+}
+
 template <int DT>
 __device__ __forceinline__ void raw8_to_float(const Raw8<DT>& r, float (&f)[8]) {
   const uint32_t w[4] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w};

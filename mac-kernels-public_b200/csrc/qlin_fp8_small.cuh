@@ -1,8 +1,8 @@
-// The block-scaled 8-bit linear for few tokens (up to 64), in one launch without a workspace.
+// The block-scaled 8-bit linear for few tokens (up to 16), in one launch without a workspace.
 //
 // With few tokens the weight's bytes are everything, so the roles of the operands are exchanged: a CTA
 // streams 128 output channels' weight tiles through TMA and multiplies them, as the MMA's 128 rows, by the
-// tokens as its columns (TN = 16, 32 or 64).  The tokens' values are quantized here, block by block
+// tokens as its TN = 16 columns.  The tokens' values are quantized here, block by block
 // beside the stream, straight into the swizzled operand tile: every CTA does it again from L2, which costs less
 // than a launch of its own and its round trip through memory.  Where the channels alone give too few CTAs to
 // keep HBM busy, a cluster of up to 8 CTAs shares the contraction and joins its sums through distributed shared
@@ -41,28 +41,28 @@ struct Fp8SmallParams {
   long long lim_x, lim_y, lim_sw;
 };
 
-template <int TN>
 struct Fp8SmallCfg {
+  static constexpr int TN = 16;
   static constexpr int kThreads = 384;
-  static constexpr int kCtas = TN == 64 ? 1 : 2;  // resident on an SM
-  static constexpr int kRing = TN == 64 ? 8 : TN == 32 ? 5 : 6;  // stages, TMEM buffers and scale slots
+  static constexpr int kCtas = 2;  // resident on an SM
+  static constexpr int kRing = 6;  // stages, TMEM buffers and scale slots
   static constexpr uint32_t kWStage = 128 * 128;
   static constexpr uint32_t kXStage = TN * 128;
-  static constexpr uint32_t kTmemCols = TN == 64 ? 512 : TN == 32 ? 256 : 128;  // at least kRing * TN
+  static constexpr uint32_t kTmemCols = 128;  // a power of two of at least kRing * TN
   static constexpr int kSmem = 1024 + kRing * (int)(kWStage + kXStage) + kRing * TN * 4 + 256;
   static_assert(kRing * TN <= kTmemCols && kCtas * kTmemCols <= 512 && kCtas * kSmem <= 228 * 1024, "resident CTAs");
   static_assert(TN * 128 * 4 <= kRing * (int)kWStage, "the joined sums fit into the weight ring");
 };
 
-// 8 consecutive values of row m from column c as they are stored, zeros past M and K.  Rows that do not take
-// 16-byte loads are gathered value by value.
+// 8 consecutive values of row m from column c as they are stored, zeros past M and K.
 template <int DT>
 __device__ __forceinline__ Raw8<DT> small_load8(const Fp8SmallParams& p, int m, int c) {
   Raw8<DT> raw{};
   const long long at = (long long)m * p.ldx + c;
   if (m >= p.M || c >= p.K) return raw;
-  if (p.x_vec && c + 8 <= p.K) {
-    if (qchk_span(BS_FP8_X, at, 8, p.lim_x)) raw = load_raw8<DT>(p.x, at);
+  if (c + 8 <= p.K) {
+    if (qchk_span(BS_FP8_X, at, 8, p.lim_x))
+      raw = p.x_vec ? load_raw8<DT>(p.x, at) : load_raw8_any<DT>(p.x, at, p.lim_x);
     return raw;
   }
   uint32_t w[DT == QLIN_F32 ? 8 : 4] = {};
@@ -83,10 +83,11 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
   return v;
 }
 
-template <int TN, bool kTrans, int DT>
-__global__ void __launch_bounds__(384, Fp8SmallCfg<TN>::kCtas)
+template <bool kTrans, int DT>
+__global__ void __launch_bounds__(384, Fp8SmallCfg::kCtas)
 fp8_small_kernel(const __grid_constant__ CUtensorMap tmap_w, const Fp8SmallParams p, int splits) {
-  using Cfg = Fp8SmallCfg<TN>;
+  using Cfg = Fp8SmallCfg;
+  constexpr int TN = Cfg::TN;
   constexpr int R = Cfg::kRing;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -274,20 +275,16 @@ fp8_small_kernel(const __grid_constant__ CUtensorMap tmap_w, const Fp8SmallParam
           !mbar_wait(&acc_full[s], ph, abort_flag, p.status, 0x58))
         break;
       tc_fence_after();
-      constexpr int kChunk = TN < 32 ? TN : 32;
+      uint32_t v[TN];
+      tmem_ld_cols<TN>(tmem_base + lanes + s * TN, v);
+      tmem_wait_ld_of(v);
 #pragma unroll
-      for (int c0 = 0; c0 < TN; c0 += kChunk) {
-        uint32_t v[kChunk];
-        tmem_ld_cols<kChunk>(tmem_base + lanes + s * TN + c0, v);
-        tmem_wait_ld_of(v);
-#pragma unroll
-        for (int j = 0; j < kChunk; j += 4) {
-          const float4 t = *reinterpret_cast<const float4*>(&scale[s * TN + c0 + j]);
-          acc[c0 + j] = fmaf(__uint_as_float(v[j]), t.x * w, acc[c0 + j]);
-          acc[c0 + j + 1] = fmaf(__uint_as_float(v[j + 1]), t.y * w, acc[c0 + j + 1]);
-          acc[c0 + j + 2] = fmaf(__uint_as_float(v[j + 2]), t.z * w, acc[c0 + j + 2]);
-          acc[c0 + j + 3] = fmaf(__uint_as_float(v[j + 3]), t.w * w, acc[c0 + j + 3]);
-        }
+      for (int j = 0; j < TN; j += 4) {
+        const float4 t = *reinterpret_cast<const float4*>(&scale[s * TN + j]);
+        acc[j] = fmaf(__uint_as_float(v[j]), t.x * w, acc[j]);
+        acc[j + 1] = fmaf(__uint_as_float(v[j + 1]), t.y * w, acc[j + 1]);
+        acc[j + 2] = fmaf(__uint_as_float(v[j + 2]), t.z * w, acc[j + 2]);
+        acc[j + 3] = fmaf(__uint_as_float(v[j + 3]), t.w * w, acc[j + 3]);
       }
       tc_fence_before();
       __syncwarp();
@@ -334,8 +331,11 @@ fp8_small_kernel(const __grid_constant__ CUtensorMap tmap_w, const Fp8SmallParam
   if (n < p.N && !aborted) {
     const float bias = fp8_bias(p.bias, p.bias_kind, n, p.N);
     for (int j = rank + splits * (warp >> 2); j < p.M; j += splits * 3) {
-      float v = bias;
-      for (int c = 0; c < splits; ++c) v += ld_cluster_f32(cluster_map(&joint[j * 128 + r], c));
+      float part[8], v = bias;  // all parts' loads in flight
+#pragma unroll
+      for (int c = 0; c < 8; ++c) part[c] = c < splits ? ld_cluster_f32(cluster_map(&joint[j * 128 + r], c)) : 0.f;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) v += c < splits ? part[c] : 0.f;
       put(j, v);
     }
   }

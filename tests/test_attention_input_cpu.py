@@ -20,7 +20,7 @@ def lib():
 
 
 def test_workspaces(lib):
-    assert lib.qlin_fp8_linear_workspace(0, 64, 128) == 0 and lib.qlin_fp8_linear_workspace(64, 64, 128) == 0 and lib.qlin_fp8_linear_workspace(4, 64, 0) == 0
+    assert lib.qlin_fp8_linear_workspace(0, 64, 128) == 0 and lib.qlin_fp8_linear_workspace(16, 64, 128) == 0 and lib.qlin_fp8_linear_workspace(4, 64, 0) == 0
     assert lib.qlin_fp8_linear_workspace(300, 64, 200) >= 300 * 256 + 2 * 300 * 4
     assert lib.qlin_fp8_linear_grad_input_workspace(300, 200, 64) >= 300 * 256 + 2 * 300 * 4
     assert lib.qlin_qk_norm_rotary_backward_workspace(0, 5, 2, 2, 64) == 0
