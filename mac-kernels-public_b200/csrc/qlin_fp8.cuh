@@ -30,6 +30,7 @@ struct Fp8Params {
   int M, N;       // tokens, output channels
   int kb;         // blocks of 128 along the contraction
   int m_tiles, n_tiles;
+  int group;        // token tiles that stay in L2 together
   const float* sx;  // [kb][ld_sx]
   long long ld_sx;
   const float* sw;  // block (output o, contraction r) at o * sw_out + r * sw_red
@@ -65,15 +66,15 @@ struct Fp8Cfg {
   static_assert(kBRows == 128, "the transposed operand is one 128-column block");
 };
 
-// Tiles in groups of kGroup token tiles, channels fastest within a group after the tokens: the tiles
-// that run at one time then share a few token tiles and a few channel tiles, which stay in L2.
-__device__ __forceinline__ void fp8_tile(int t, int m_tiles, int n_tiles, int& mt, int& nt) {
-  constexpr int kGroup = 8;
-  const int per = kGroup * n_tiles;
+// Tiles in groups of `group` token tiles, tokens fastest and then channels within a group: the tiles that run at
+// one time share a few token tiles and a few channel tiles, and a group's tokens stay in L2 while the channels
+// stream past them.
+__device__ __forceinline__ void fp8_tile(int t, int m_tiles, int n_tiles, int group, int& mt, int& nt) {
+  const int per = group * n_tiles;
   const int g = t / per, r = t - g * per;
-  const int rows = min(kGroup, m_tiles - g * kGroup);
+  const int rows = min(group, m_tiles - g * group);
   nt = r / rows;
-  mt = g * kGroup + (r - nt * rows);
+  mt = g * group + (r - nt * rows);
 }
 
 // Pitch of a token's sums in shared memory, in floats: 16 bytes past a multiple of 128, so that the lanes of a
@@ -198,7 +199,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
         bool ok = true;
         for (int t = tile0; t < num_tiles && ok; t += tile_step) {
           int mt, nt;
-          fp8_tile(t, p.m_tiles, p.n_tiles, mt, nt);
+          fp8_tile(t, p.m_tiles, p.n_tiles, p.group, mt, nt);
           const int m0 = (mt * CTAS + (int)rank) * 128;
           const int n0 = nt * TN + (int)rank * Cfg::kBRows;
           for (int b = b_begin; b < b_end; ++b, ++it) {
@@ -290,7 +291,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
     bool ok = true;
     for (int t = tile0; t < num_tiles && ok; t += tile_step) {
       int mt, nt;
-      fp8_tile(t, p.m_tiles, p.n_tiles, mt, nt);
+      fp8_tile(t, p.m_tiles, p.n_tiles, p.group, mt, nt);
       const int m = (mt * CTAS + (int)rank) * 128 + r;
       const int n0 = nt * TN + part * kCols;  // kCols channels from here, inside one 128-channel block
       const long long sw_off = (long long)min(n0 / 128, (p.N - 1) / 128) * p.sw_out;
@@ -449,7 +450,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
       cluster_sync();
       const bool aborted = *abort_flag != 0;
       int mt, nt;
-      fp8_tile(tile0, p.m_tiles, p.n_tiles, mt, nt);
+      fp8_tile(tile0, p.m_tiles, p.n_tiles, p.group, mt, nt);
       const int n = nt * TN + lane * 4;
       const int valid = min(128, p.M - mt * 128);
       constexpr int kWarps = Cfg::kEpiWarps;
