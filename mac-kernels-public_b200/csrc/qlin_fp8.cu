@@ -28,7 +28,7 @@ struct QuantFp8Params {
   const void* x;
   long long ldx;
   int M, K, kb;      // kb = blocks of 128, the last one padded with zeros
-  int k_tiles;       // CTAs along the blocks
+  int k_pairs;       // pairs of blocks
   uint8_t* q;
   long long ldq;
   float* scale;      // [kb][ld_scale]
@@ -36,25 +36,89 @@ struct QuantFp8Params {
   long long lim_x, lim_q, lim_scale;  // element counts for the QLIN_CHECKS build
 };
 
+// The w-th aligned 16-byte word around address at; zeros from the row's end on.  A word that reaches past the caller's
+// values [base, end) is read value by value.
+template <int kBytes>
+__device__ __forceinline__ uint4 aligned_word(const uint8_t* at, int w, const uint8_t* row_end, const uint8_t* base,
+                                              const uint8_t* end) {
+  const uint8_t* from = reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(at) & ~uintptr_t(15)) + w * 16;
+  if (from >= row_end) return uint4{};
+  if (from >= base && from + 16 <= end) return __ldg(reinterpret_cast<const uint4*>(from));
+  uint32_t o[4] = {};
+#pragma unroll
+  for (int j = 0; j < 16 / kBytes; ++j) {
+    const uint8_t* e = from + j * kBytes;
+    if (e < base || e >= end) continue;
+    if constexpr (kBytes == 4) o[j] = *reinterpret_cast<const uint32_t*>(e);
+    else o[j / 2] |= (uint32_t) * reinterpret_cast<const uint16_t*>(e) << (16 * (j & 1));
+  }
+  return make_uint4(o[0], o[1], o[2], o[3]);
+}
+
 template <int DT, bool kVec>
 __global__ void __launch_bounds__(256) quant_rows_fp8_kernel(const QuantFp8Params p) {
   constexpr int kRows = 8;
   griddep_launch();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int row_tile = blockIdx.x / p.k_tiles;
-  const int b = ((blockIdx.x - row_tile * p.k_tiles) * 8 + warp) * 2 + (lane >> 4);
+  const uint32_t item = blockIdx.x * 8u + warp;  // a warp takes 8 rows of two blocks; neighbours the next blocks
+  const int row_tile = (int)(item / (uint32_t)p.k_pairs);
+  const int b = (int)(item - (uint32_t)row_tile * (uint32_t)p.k_pairs) * 2 + (lane >> 4);
   const int m0 = row_tile * kRows;
+  if (m0 >= p.M) return;
   const int c = b * 128 + (lane & 15) * 8;
   const int rows = min(kRows, p.M - m0);
   float f[kRows][8];
-  if (c + 8 <= p.K) {
+  if constexpr (!kVec) {
+    // Rows that start off a 16-byte boundary: every lane reads the aligned words its values begin in, and takes
+    // what they end in from the next lane; the words after the last lane's are read by a lane for each row.
+    constexpr int kBytes = DT == QLIN_F32 ? 4 : 2;
+    constexpr int kOwn = kBytes / 2;  // words of 16 bytes
+    const int b0 = b - (lane >> 4);
+    const uint8_t* base = reinterpret_cast<const uint8_t*>(p.x);
+    const uint8_t* end = base + p.lim_x * kBytes;
+    uint4 own[kRows][kOwn];
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      const uint8_t* row = base + (long long)(m0 + min(i, rows - 1)) * p.ldx * kBytes;
+#pragma unroll
+      for (int w = 0; w < kOwn; ++w)
+        own[i][w] = aligned_word<kBytes>(row + (long long)c * kBytes, w, row + (long long)p.K * kBytes, base, end);
+    }
+    const uint8_t* my_row = base + (long long)(m0 + min(lane & 7, rows - 1)) * p.ldx * kBytes;
+    const uint4 past = lane < 8 ? aligned_word<kBytes>(my_row + (b0 * 128ll + 256) * kBytes, 0,
+                                                       my_row + (long long)p.K * kBytes, base, end)
+                                : uint4{};
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      Around8<DT> a;
+      const uint8_t* at = base + ((long long)(m0 + min(i, rows - 1)) * p.ldx + c) * kBytes;
+      a.off = (uint32_t)(reinterpret_cast<uintptr_t>(at) & 15);
+#pragma unroll
+      for (int w = 0; w < kOwn; ++w) a.v[w] = own[i][w];
+      uint4 next;
+      next.x = __shfl_down_sync(0xffffffffu, own[i][0].x, 1);
+      next.y = __shfl_down_sync(0xffffffffu, own[i][0].y, 1);
+      next.z = __shfl_down_sync(0xffffffffu, own[i][0].z, 1);
+      next.w = __shfl_down_sync(0xffffffffu, own[i][0].w, 1);
+      uint4 last;
+      last.x = __shfl_sync(0xffffffffu, past.x, i);
+      last.y = __shfl_sync(0xffffffffu, past.y, i);
+      last.z = __shfl_sync(0xffffffffu, past.z, i);
+      last.w = __shfl_sync(0xffffffffu, past.w, i);
+      a.v[kOwn] = lane == 31 ? last : next;
+      raw8_to_float<DT>(a.values(), f[i]);
+      if (c + 8 > p.K) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[i][j] = c + j < p.K ? f[i][j] : 0.f;
+      }
+    }
+  } else if (c + 8 <= p.K) {
     Raw8<DT> raw[kRows];
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
       const long long at = (long long)(m0 + min(i, rows - 1)) * p.ldx + c;
       raw[i] = Raw8<DT>{};
-      if (qchk_span(BS_FP8_QUANT, at, 8, p.lim_x))
-        raw[i] = kVec ? load_raw8<DT>(p.x, at) : load_raw8_any<DT>(p.x, at, p.lim_x);
+      if (qchk_span(BS_FP8_QUANT, at, 8, p.lim_x)) raw[i] = load_raw8<DT>(p.x, at);
     }
 #pragma unroll
     for (int i = 0; i < kRows; ++i) raw8_to_float<DT>(raw[i], f[i]);
@@ -113,7 +177,7 @@ static int launch_quant_rows_fp8(const void* x, int x_dtype, long long ldx, int 
   p.M = M;
   p.K = K;
   p.kb = (K + 127) / 128;
-  p.k_tiles = (p.kb + 15) / 16;
+  p.k_pairs = (p.kb + 1) / 2;
   p.q = q;
   p.ldq = ldq;
   p.scale = scale;
@@ -121,8 +185,8 @@ static int launch_quant_rows_fp8(const void* x, int x_dtype, long long ldx, int 
   p.lim_x = (long long)(M - 1) * ldx + K;
   p.lim_q = (long long)(M - 1) * ldq + (long long)p.kb * 128;
   p.lim_scale = (long long)(p.kb - 1) * ld_scale + M;
-  const long long grid = (long long)((M + 7) / 8) * p.k_tiles;
-  if (grid > 0x7fffffff) {
+  const long long grid = ((long long)((M + 7) / 8) * p.k_pairs + 7) / 8;
+  if (grid > 0x7fffffff / 8) {
     set_error("fp8 quantizer: %d rows of %d columns are too many", M, K);
     return QLIN_EINVAL;
   }

@@ -15,8 +15,8 @@
 // Warp roles (384 threads, one CTA per SM, persistent over the tiles):
 //   warp 0        TMA producer            warp 1   TMEM alloc + MMA issuer       (warps 2, 3 idle)
 //   warps 4..11   rescale + epilogue: two warps per TMEM lane quarter, half the columns each
-// The epilogue warps take over most of the first warpgroup's registers: a pair's warp holds 128 running
-// sums and two loads of 32 values.
+// A pair's epilogue warps hold 128 running sums a thread and take over most of the first warpgroup's
+// registers.
 #pragma once
 #include <cuda.h>
 
@@ -59,7 +59,8 @@ struct Fp8Cfg {
   static constexpr uint32_t kBStage = kBRows * 128;
   static constexpr int kStages = 5;
   static constexpr int kCols = TN / (kEpiWarps / 4);  // accumulator columns per epilogue warp
-  static constexpr uint32_t kOutWarp = 32 * kCols * 2;  // output staging of a warp: its tokens' rows, 2 bytes a value
+  // output staging of a warp: its tokens' rows, 2 bytes a value, or one piece of them with kOddPitch
+  static constexpr uint32_t kOutWarp = kCols == 128 ? 32 * 256 : 5 * 1024;
   static constexpr int kSmem = 1024 + kStages * (int)(kAStage + kBStage) + kEpiWarps * (int)kOutWarp + 512;
   static_assert(CTAS == 1 || CTAS == 2, "one CTA or a pair");
   static_assert(128 * 132 * 4 <= kStages * (int)(kAStage + kBStage), "the joined sums fit over the operand ring");
@@ -116,6 +117,52 @@ __device__ __forceinline__ uint32_t pack_out2(int dtype, float a, float b) {
   }
   const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Pitch of a row's piece staged at its address modulo 16: 128 bytes after an offset of up to 14.
+constexpr int kOddPitch = 144;
+
+// Where a row's bytes from address g on reach 16-byte boundaries: the first one, and the whole words from there.
+struct OddRow {
+  int head, body;
+  __device__ __forceinline__ OddRow(const uint8_t* g, int bytes) {
+    head = (16 - (int)(reinterpret_cast<uintptr_t>(g) & 15)) & 15;
+    body = bytes > head ? (bytes - head) & ~15 : 0;
+  }
+};
+
+// What lies before the first and after the last whole 16-byte word of a row's bytes at g, from shared memory (same
+// address modulo 16): at most three stores at each end.
+template <int kBytes>
+__device__ __forceinline__ void store_odd_ends(uint8_t* g, const uint8_t* s, int bytes, const OddRow& o) {
+  if (bytes <= o.head) {  // a few columns at the end of y
+    for (int i = 0; i < bytes; i += kBytes) {
+      if constexpr (kBytes == 2) *reinterpret_cast<uint16_t*>(g + i) = *reinterpret_cast<const uint16_t*>(s + i);
+      else *reinterpret_cast<uint32_t*>(g + i) = *reinterpret_cast<const uint32_t*>(s + i);
+    }
+    return;
+  }
+  int i = 0;
+  if (kBytes == 2 && (o.head & 2)) {
+    *reinterpret_cast<uint16_t*>(g) = *reinterpret_cast<const uint16_t*>(s);
+    i = 2;
+  }
+  if (o.head & 4) {
+    *reinterpret_cast<uint32_t*>(g + i) = *reinterpret_cast<const uint32_t*>(s + i);
+    i += 4;
+  }
+  if (o.head & 8) *reinterpret_cast<uint2*>(g + i) = *reinterpret_cast<const uint2*>(s + i);
+  i = o.head + o.body;
+  const int tail = bytes - i;
+  if (tail & 8) {
+    *reinterpret_cast<uint2*>(g + i) = *reinterpret_cast<const uint2*>(s + i);
+    i += 8;
+  }
+  if (tail & 4) {
+    *reinterpret_cast<uint32_t*>(g + i) = *reinterpret_cast<const uint32_t*>(s + i);
+    i += 4;
+  }
+  if (kBytes == 2 && (tail & 2)) *reinterpret_cast<uint16_t*>(g + i) = *reinterpret_cast<const uint16_t*>(s + i);
 }
 
 template <int CTAS, int TN, bool kTrans>
@@ -188,9 +235,9 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
   const uint32_t tmem_base = *tmem_slot;
   griddep_wait();  // the quantizer's codes and scales
 
-  // setmaxnreg: 2 x 224 + 56 = 3 x 168, the registers of an SM quarter's three warps at launch
+  // setmaxnreg (pairs): 2 x 224 + 56 = 3 x 168, the registers of an SM quarter's three warps at launch
   if (warp < 4) {
-    setmaxnreg_dec<56>();
+    if constexpr (CTAS == 2) setmaxnreg_dec<56>();
     if (warp == 0) {
       // --------------------------------------------------------------------- producer (both CTAs)
       if (elect_one()) {
@@ -278,7 +325,7 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
       cluster_sync();
     }
   } else {
-    setmaxnreg_inc<224>();
+    if constexpr (CTAS == 2) setmaxnreg_inc<224>();
     // --------------------------------------------------------------------- rescale + epilogue
     constexpr int kCols = Cfg::kCols;
     constexpr int kChunk = 16;
@@ -371,13 +418,15 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
         }
         break;
       }
-      // The warp's 32 rows go through its own staging buffer, 128 bytes of each row at a time, 16-byte pieces
-      // swizzled by the row; they leave as TMA stores (clipped at M and N), which the next tile's products
-      // do not wait for, or, where y's rows are not 16-byte aligned, as plain stores along the rows.
+      // The warp's 32 rows go through its own staging buffer, 128 bytes of each row at a time.  Where y's rows are
+      // 16-byte aligned they leave as TMA stores, which the next tile's products do not wait for,
+      // clipped at M and N, the 16-byte pieces swizzled by the row.  Else a row is staged at its global address
+      // modulo 16, so that all but its first and last bytes leave in 16-byte stores, 8 lanes to a row.  (A bulk copy
+      // for each row and piece, 1024 a tile in fp32, took longer than the tile's products.)
       const int m_warp = (mt * CTAS + (int)rank) * 128 + quarter * 32;
       uint8_t* stage = so + (warp - 4) * Cfg::kOutWarp;
       constexpr int kPieceBytes = 32 * 128;
-      constexpr int kPieces = Cfg::kOutWarp / kPieceBytes;
+      constexpr int kPieces = kCols == 128 ? 2 : 1;
       bool used[kPieces] = {};
       const bool wide = p.y_dtype == OUT_F32;
       if (lane == 0) bulk_wait_read<0>();  // the last tile's stores have left the buffer
@@ -385,9 +434,51 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
       auto piece = [&](auto wide_c, int c0) {  // 128 bytes of every row: the values from column c0
         constexpr bool kWide = decltype(wide_c)::value;
         constexpr int kN = kWide ? 32 : 64;
+        const int n = n0 + c0;
+        if (!p.tma_out) {
+          constexpr int kBytes = kWide ? 4 : 2;
+          const int bytes = min(kN, p.N - n) * kBytes;
+          uint8_t* g0 = reinterpret_cast<uint8_t*>(p.y) + ((long long)m_warp * p.ldy + n) * kBytes;
+          const long long pitch = p.ldy * kBytes;
+          if (bytes <= 0 || !qchk_smem(BS_FP8_SMEM, smem_raw, stage, 32 * kOddPitch)) return;
+          __syncwarp();  // the last piece has left
+          uint8_t* g = g0 + lane * pitch;
+          uint8_t* row = stage + lane * kOddPitch;
+          const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(g) & 15);
+          if constexpr (kWide) {
+#pragma unroll
+            for (int j = 0; j < kN; ++j) *reinterpret_cast<float*>(row + off + 4 * j) = acc[c0 + j];
+          } else {
+            uint32_t last = 0;
+            const bool odd = off & 2;
+#pragma unroll
+            for (int j = 0; j < kN / 2; ++j) {
+              const uint32_t w = pack_out2(p.y_dtype, acc[c0 + 2 * j], acc[c0 + 2 * j + 1]);
+              *reinterpret_cast<uint32_t*>(row + (off & 12) + 4 * j) = odd ? __funnelshift_l(last, w, 16) : w;
+              last = w;
+            }
+            if (odd) *reinterpret_cast<uint16_t*>(row + (off & 12) + 2 * kN) = (uint16_t)(last >> 16);
+          }
+          __syncwarp();
+          const int rows = min(32, p.M - m_warp);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {  // 8 lanes to a row, 4 rows at a time
+            const int rr = i * 4 + (lane >> 3), word = (lane & 7) * 16;
+            uint8_t* gr = g0 + rr * pitch;
+            const OddRow o(gr, bytes);
+            const int at = o.head + word;
+            if (rr < rows && word < o.body &&
+                qchk_span(BS_FP8_Y, (gr + at - reinterpret_cast<uint8_t*>(p.y)) / kBytes, 16 / kBytes, p.lim_y))
+              *reinterpret_cast<uint4*>(gr + at) = *reinterpret_cast<const uint4*>(
+                  stage + rr * kOddPitch + (reinterpret_cast<uintptr_t>(gr) & 15) + at);
+          }
+          if (lane < rows && qchk_span(BS_FP8_Y, (g - reinterpret_cast<uint8_t*>(p.y)) / kBytes, bytes / kBytes, p.lim_y))
+            store_odd_ends<kBytes>(g, row + off, bytes, OddRow(g, bytes));
+          return;
+        }
         const int slot = (c0 / kN) % kPieces;
         uint8_t* dst = stage + slot * kPieceBytes;
-        if (used[slot]) {  // fp32 only: the buffer holds half of the row
+        if (used[slot]) {  // the buffer holds a part of the row
           if (lane == 0) bulk_wait_read<0>();
           __syncwarp();
         }
@@ -408,31 +499,11 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
             *reinterpret_cast<uint4*>(dst + lane * 128 + ((ch ^ (lane & 7)) << 4)) = w;
           }
         }
-        const int n = n0 + c0;
-        if (p.tma_out) {
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            if (n < p.N && m_warp < p.M) tma_store_2d(&tmap_y, dst, n, m_warp);
-            bulk_commit();
-          }
-        } else {
-          __syncwarp();
-          const int rows = min(32, p.M - m_warp);
-#pragma unroll 4
-          for (int rr = 0; rr < rows; ++rr) {
-#pragma unroll
-            for (int q = 0; q < kN / 32; ++q) {
-              const int j = q * 32 + lane;
-              const int byte = kWide ? j * 4 : j * 2;
-              const uint8_t* src = dst + rr * 128 + ((((byte >> 4) ^ (rr & 7)) << 4) | (byte & 15));
-              const long long at = (long long)(m_warp + rr) * p.ldy + n + j;
-              if (n + j >= p.N || !qchk(BS_FP8_Y, at, p.lim_y)) continue;
-              if constexpr (kWide) reinterpret_cast<float*>(p.y)[at] = *reinterpret_cast<const float*>(src);
-              else reinterpret_cast<uint16_t*>(p.y)[at] = *reinterpret_cast<const uint16_t*>(src);
-            }
-          }
-          __syncwarp();
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          if (n < p.N && m_warp < p.M) tma_store_2d(&tmap_y, dst, n, m_warp);
+          bulk_commit();
         }
       };
       if (wide) {

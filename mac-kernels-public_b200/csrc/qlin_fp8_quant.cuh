@@ -34,45 +34,74 @@ __device__ __forceinline__ Raw8<DT> load_raw8(const void* x, long long i) {
   return r;
 }
 
-// The same from any address of the type's alignment: the aligned 16-byte words around the values, shifted.
-// `lim` is the number of values from x on that are the caller's; where the words reach past them, value by value.
+// The same from any address of the type's alignment: the aligned 16-byte words around the values (load), shifted
+// when they have arrived (values).  `lim` is the number of values from x on that are the caller's; where the words
+// would reach past them, the values are read one by one.
 template <int DT>
-__device__ __forceinline__ Raw8<DT> load_raw8_any(const void* x, long long i, long long lim) {
-  constexpr int kBytes = DT == QLIN_F32 ? 4 : 2;
-  constexpr int kWords = DT == QLIN_F32 ? 12 : 8;  // 32-bit words read
-  constexpr int kOut = DT == QLIN_F32 ? 8 : 4;
-  const uintptr_t at = reinterpret_cast<uintptr_t>(x) + i * kBytes;
-  const uintptr_t from = at & ~uintptr_t(15);
-  uint32_t o[kOut] = {};
-  if (from >= reinterpret_cast<uintptr_t>(x) && from + kWords * 4 <= reinterpret_cast<uintptr_t>(x) + lim * kBytes) {
+struct Around8 {
+  static constexpr int kBytes = DT == QLIN_F32 ? 4 : 2;
+  static constexpr int kWords = DT == QLIN_F32 ? 12 : 8;  // 32-bit words read
+  static constexpr int kOut = DT == QLIN_F32 ? 8 : 4;
+  uint4 v[kWords / 4];
+  uint32_t off;  // of the values, in bytes from v; 16: the values lie in v as they are
+
+  __device__ __forceinline__ void load(const void* x, long long i, long long lim) {
+    const uintptr_t begin = reinterpret_cast<uintptr_t>(x), at = begin + i * kBytes, from = at & ~uintptr_t(15);
+    const bool inside = from >= begin && from + kWords * 4 <= begin + lim * kBytes;
+    off = inside ? (uint32_t)(at & 15) : 16;
+#pragma unroll
+    for (int j = 0; j < kWords / 4; ++j) v[j] = inside ? __ldg(reinterpret_cast<const uint4*>(from) + j) : uint4{};
+    if (!inside) {
+      uint32_t o[kWords] = {};
+      for (int j = 0; j < 8; ++j) {
+        if constexpr (DT == QLIN_F32) {
+          const uint32_t b = reinterpret_cast<const uint32_t*>(x)[i + j];
+#pragma unroll
+          for (int q = 0; q < 8; ++q) o[q] = q == j ? b : o[q];
+        } else {
+          const uint32_t b = (uint32_t) reinterpret_cast<const uint16_t*>(x)[i + j] << (16 * (j & 1));
+#pragma unroll
+          for (int q = 0; q < 4; ++q) o[q] |= q == j / 2 ? b : 0;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kWords / 4; ++j) v[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+    }
+  }
+  __device__ __forceinline__ void clear() {
+    off = 16;
+#pragma unroll
+    for (int j = 0; j < kWords / 4; ++j) v[j] = uint4{};
+  }
+  __device__ __forceinline__ Raw8<DT> values() const {
     uint32_t w[kWords + 1];
 #pragma unroll
     for (int j = 0; j < kWords / 4; ++j) {
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(from) + j);
-      w[4 * j] = v.x;
-      w[4 * j + 1] = v.y;
-      w[4 * j + 2] = v.z;
-      w[4 * j + 3] = v.w;
+      w[4 * j] = v[j].x;
+      w[4 * j + 1] = v[j].y;
+      w[4 * j + 2] = v[j].z;
+      w[4 * j + 3] = v[j].w;
     }
     w[kWords] = 0;
-    const uint32_t off = (uint32_t)(at & 15);
 #pragma unroll
     for (int j = 0; j + 2 <= kWords; ++j) w[j] = (off & 8) ? w[j + 2] : w[j];
 #pragma unroll
     for (int j = 0; j + 1 <= kWords; ++j) w[j] = (off & 4) ? w[j + 1] : w[j];
+    uint32_t o[kOut];
 #pragma unroll
     for (int j = 0; j < kOut; ++j) o[j] = kBytes == 2 ? __funnelshift_r(w[j], w[j + 1], (off & 2) * 8) : w[j];
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if constexpr (DT == QLIN_F32) o[j] = reinterpret_cast<const uint32_t*>(x)[i + j];
-      else o[j / 2] |= (uint32_t) reinterpret_cast<const uint16_t*>(x)[i + j] << (16 * (j & 1));
-    }
+    Raw8<DT> r;
+    r.v[0] = make_uint4(o[0], o[1], o[2], o[3]);
+    if constexpr (DT == QLIN_F32) r.v[1] = make_uint4(o[4], o[5], o[6], o[7]);
+    return r;
   }
-  Raw8<DT> r;
-  r.v[0] = make_uint4(o[0], o[1], o[2], o[3]);
-  if constexpr (DT == QLIN_F32) r.v[1] = make_uint4(o[4], o[5], o[6], o[7]);
-  return r;
+};
+
+template <int DT>
+__device__ __forceinline__ Raw8<DT> load_raw8_any(const void* x, long long i, long long lim) {
+  Around8<DT> a;
+  a.load(x, i, lim);
+  return a.values();
 }
 
 template <int DT>
