@@ -119,23 +119,14 @@ __device__ __forceinline__ uint32_t pack_out2(int dtype, float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Pitch of a row's piece staged at its address modulo 16: 128 bytes after an offset of up to 14.
+// Pitch of a staged row's piece: 8 words of 16 bytes and, behind the last piece, what is left of the row.
 constexpr int kOddPitch = 144;
 
-// Where a row's bytes from address g on reach 16-byte boundaries: the first one, and the whole words from there.
-struct OddRow {
-  int head, body;
-  __device__ __forceinline__ OddRow(const uint8_t* g, int bytes) {
-    head = (16 - (int)(reinterpret_cast<uintptr_t>(g) & 15)) & 15;
-    body = bytes > head ? (bytes - head) & ~15 : 0;
-  }
-};
-
-// What lies before the first and after the last whole 16-byte word of a row's bytes at g, from shared memory (same
-// address modulo 16): at most three stores at each end.
+// The first bytes of a row, up to a 16-byte boundary (or its end before that), and the last ones, from a boundary
+// on, from shared memory at the same address modulo 16.
 template <int kBytes>
-__device__ __forceinline__ void store_odd_ends(uint8_t* g, const uint8_t* s, int bytes, const OddRow& o) {
-  if (bytes <= o.head) {  // a few columns at the end of y
+__device__ __forceinline__ void store_head(uint8_t* g, const uint8_t* s, int bytes) {
+  if (((reinterpret_cast<uintptr_t>(g) + bytes) & 15) != 0) {  // a few columns at the end of y
     for (int i = 0; i < bytes; i += kBytes) {
       if constexpr (kBytes == 2) *reinterpret_cast<uint16_t*>(g + i) = *reinterpret_cast<const uint16_t*>(s + i);
       else *reinterpret_cast<uint32_t*>(g + i) = *reinterpret_cast<const uint32_t*>(s + i);
@@ -143,26 +134,28 @@ __device__ __forceinline__ void store_odd_ends(uint8_t* g, const uint8_t* s, int
     return;
   }
   int i = 0;
-  if (kBytes == 2 && (o.head & 2)) {
+  if (kBytes == 2 && (bytes & 2)) {
     *reinterpret_cast<uint16_t*>(g) = *reinterpret_cast<const uint16_t*>(s);
     i = 2;
   }
-  if (o.head & 4) {
+  if (bytes & 4) {
     *reinterpret_cast<uint32_t*>(g + i) = *reinterpret_cast<const uint32_t*>(s + i);
     i += 4;
   }
-  if (o.head & 8) *reinterpret_cast<uint2*>(g + i) = *reinterpret_cast<const uint2*>(s + i);
-  i = o.head + o.body;
-  const int tail = bytes - i;
-  if (tail & 8) {
-    *reinterpret_cast<uint2*>(g + i) = *reinterpret_cast<const uint2*>(s + i);
-    i += 8;
+  if (bytes & 8) *reinterpret_cast<uint2*>(g + i) = *reinterpret_cast<const uint2*>(s + i);
+}
+template <int kBytes>
+__device__ __forceinline__ void store_tail(uint8_t* g, const uint8_t* s, int bytes) {
+  int i = 0;
+  if (bytes & 8) {
+    *reinterpret_cast<uint2*>(g) = *reinterpret_cast<const uint2*>(s);
+    i = 8;
   }
-  if (tail & 4) {
+  if (bytes & 4) {
     *reinterpret_cast<uint32_t*>(g + i) = *reinterpret_cast<const uint32_t*>(s + i);
     i += 4;
   }
-  if (kBytes == 2 && (tail & 2)) *reinterpret_cast<uint16_t*>(g + i) = *reinterpret_cast<const uint16_t*>(s + i);
+  if (kBytes == 2 && (bytes & 2)) *reinterpret_cast<uint16_t*>(g + i) = *reinterpret_cast<const uint16_t*>(s + i);
 }
 
 template <int CTAS, int TN, bool kTrans>
@@ -436,44 +429,60 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
         constexpr int kN = kWide ? 32 : 64;
         const int n = n0 + c0;
         if (!p.tma_out) {
+          // The row in 32-bit words, shifted in registers to its address modulo 16: word j of this piece is what
+          // belongs at the row's first 16-byte boundary at or below its start, plus 4 (w0 + j).
           constexpr int kBytes = kWide ? 4 : 2;
-          const int bytes = min(kN, p.N - n) * kBytes;
-          uint8_t* g0 = reinterpret_cast<uint8_t*>(p.y) + ((long long)m_warp * p.ldy + n) * kBytes;
+          const int w0 = c0 * kBytes / 4;
+          const bool last_piece = c0 + kN == kCols;
+          const int bytes = min(kCols, p.N - n0) * kBytes;  // of the row's part that this warp has
+          uint8_t* g0 = reinterpret_cast<uint8_t*>(p.y) + ((long long)m_warp * p.ldy + n0) * kBytes;
           const long long pitch = p.ldy * kBytes;
           if (bytes <= 0 || !qchk_smem(BS_FP8_SMEM, smem_raw, stage, 32 * kOddPitch)) return;
-          __syncwarp();  // the last piece has left
           uint8_t* g = g0 + lane * pitch;
           uint8_t* row = stage + lane * kOddPitch;
-          const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(g) & 15);
-          if constexpr (kWide) {
+          const int off = (int)(reinterpret_cast<uintptr_t>(g) & 15);
+          uint32_t r[40];  // words w0 - 4 .. w0 + 35
 #pragma unroll
-            for (int j = 0; j < kN; ++j) *reinterpret_cast<float*>(row + off + 4 * j) = acc[c0 + j];
-          } else {
-            uint32_t last = 0;
-            const bool odd = off & 2;
-#pragma unroll
-            for (int j = 0; j < kN / 2; ++j) {
-              const uint32_t w = pack_out2(p.y_dtype, acc[c0 + 2 * j], acc[c0 + 2 * j + 1]);
-              *reinterpret_cast<uint32_t*>(row + (off & 12) + 4 * j) = odd ? __funnelshift_l(last, w, 16) : w;
-              last = w;
-            }
-            if (odd) *reinterpret_cast<uint16_t*>(row + (off & 12) + 2 * kN) = (uint16_t)(last >> 16);
+          for (int k = 0; k < 40; ++k) {
+            const int j = w0 + k - 4;
+            if (j < 0 || k >= 36 || j * 4 / kBytes >= kCols) r[k] = 0;
+            else if constexpr (kWide) r[k] = __float_as_uint(acc[j]);
+            else r[k] = pack_out2(p.y_dtype, acc[2 * j], acc[2 * j + 1]);
           }
+          if constexpr (!kWide) {
+#pragma unroll
+            for (int k = 39; k > 0; --k) r[k] = (off & 2) ? __funnelshift_l(r[k - 1], r[k], 16) : r[k];
+          }
+#pragma unroll
+          for (int k = 39; k > 1; --k) r[k] = (off & 4) ? r[k - 1] : r[k];
+#pragma unroll
+          for (int k = 39; k > 3; --k) r[k] = (off & 8) ? r[k - 2] : r[k];
+          __syncwarp();  // the last piece has left
+#pragma unroll
+          for (int w = 0; w < 9; ++w)
+            if (w < 8 || last_piece)
+              *reinterpret_cast<uint4*>(row + w * 16) = make_uint4(r[4 * w + 4], r[4 * w + 5], r[4 * w + 6], r[4 * w + 7]);
           __syncwarp();
           const int rows = min(32, p.M - m_warp);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {  // 8 lanes to a row, 4 rows at a time
-            const int rr = i * 4 + (lane >> 3), word = (lane & 7) * 16;
+            const int rr = i * 4 + (lane >> 3), w = lane & 7;
             uint8_t* gr = g0 + rr * pitch;
-            const OddRow o(gr, bytes);
-            const int at = o.head + word;
-            if (rr < rows && word < o.body &&
-                qchk_span(BS_FP8_Y, (gr + at - reinterpret_cast<uint8_t*>(p.y)) / kBytes, 16 / kBytes, p.lim_y))
-              *reinterpret_cast<uint4*>(gr + at) = *reinterpret_cast<const uint4*>(
-                  stage + rr * kOddPitch + (reinterpret_cast<uintptr_t>(gr) & 15) + at);
+            const int o = (int)(reinterpret_cast<uintptr_t>(gr) & 15), rel = w0 * 4 + w * 16;
+            if (rr < rows && rel >= o && rel + 16 <= o + bytes &&
+                qchk_span(BS_FP8_Y, (gr - o + rel - reinterpret_cast<uint8_t*>(p.y)) / kBytes, 16 / kBytes, p.lim_y))
+              *reinterpret_cast<uint4*>(gr - o + rel) = *reinterpret_cast<const uint4*>(stage + rr * kOddPitch + w * 16);
           }
-          if (lane < rows && qchk_span(BS_FP8_Y, (g - reinterpret_cast<uint8_t*>(p.y)) / kBytes, bytes / kBytes, p.lim_y))
-            store_odd_ends<kBytes>(g, row + off, bytes, OddRow(g, bytes));
+          if (lane < rows) {
+            const int end = off + bytes, tail = end & ~15;
+            if (c0 == 0 && off > 0 &&
+                qchk_span(BS_FP8_Y, (g - reinterpret_cast<uint8_t*>(p.y)) / kBytes, (min(16, end) - off) / kBytes, p.lim_y))
+              store_head<kBytes>(g, row + off, min(16, end) - off);
+            const int in = tail - w0 * 4;  // where the row's last word lies in this piece
+            if (end > tail && in >= 0 && in < (last_piece ? 144 : 128) && (tail > 0 || off == 0) &&
+                qchk_span(BS_FP8_Y, (g - off + tail - reinterpret_cast<uint8_t*>(p.y)) / kBytes, (end - tail) / kBytes, p.lim_y))
+              store_tail<kBytes>(g - off + tail, row + in, end - tail);
+          }
           return;
         }
         const int slot = (c0 / kN) % kPieces;
