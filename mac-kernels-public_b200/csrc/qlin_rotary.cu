@@ -381,11 +381,12 @@ __global__ void __launch_bounds__(256, 4) qk_norm_rotary_kernel(const __grid_con
 // Backward.  The CTAs of a side walk over its (token, share of heads) items; every lane sums its 8 columns'
 // g * xhat in fp32, the CTA joins its rows in a fixed order and leaves one partial row of dw, and the
 // kernel below adds those up, also in a fixed order.
+__host__ __device__ constexpr int bwd_unroll(int dtype) { return dtype == QLIN_F32 ? 2 : 3; }
 constexpr int kBwdCtas = 2;  // resident on an SM: 128 registers a thread
 template <int DT, int G, bool kInter>
 __global__ void __launch_bounds__(256, kBwdCtas) qk_norm_rotary_bwd_kernel(const __grid_constant__ HeadParams p) {
   constexpr int R = 32 / G;
-  constexpr int kUnroll = DT == QLIN_F32 ? 2 : 3;
+  constexpr int kUnroll = bwd_unroll(DT);
   __shared__ float part[8 * R][G * 8];
   griddep_launch();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -398,70 +399,93 @@ __global__ void __launch_bounds__(256, kBwdCtas) qk_norm_rotary_bwd_kernel(const
 #pragma unroll
   for (int j = 0; j < 8; ++j) dw[j] = 0.f;
   const float inv_d = 1.f / (float)p.D;
-  const long long items = p.tokens * sd.chunks;
-  for (long long item = (long long)cta * 8 + warp; item < items; item += (long long)p.ctas[which] * 8) {
+  const long long items = p.tokens * sd.chunks, stride = (long long)p.ctas[which] * 8;
+  long long item = (long long)cta * 8 + warp;
+  // The rows that are loaded ahead: of the same token, or the first ones of the warp's next.
+  long long xr = 0, yr = 0, gr = 0;
+  int h0 = 0, h_end = 0;
+  float c_next[4], s_next[4];
+  Pieces<DT> rx[kUnroll], rg[kUnroll];
+  auto begin_item = [&]() {
     const long long token = sd.chunks == 1 ? item : item / sd.chunks;
     const int chunk = (int)(item - token * sd.chunks);
     long long b, l;
     token_of(p, token, b, l);
+    load_turn(p, b * p.table_b + l * p.pairs, plan.pair0, c_next, s_next);
+    xr = b * sd.x_b + l * sd.x_l;
+    yr = b * sd.y_b + l * sd.y_l;
+    gr = b * sd.dy_b + l * sd.dy_l;
+    h0 = chunk * p.heads_per_warp;
+    h_end = min(sd.heads, h0 + p.heads_per_warp);
+  };
+  auto load = [&]() {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int h = h0 + u * R + lane / G;
+      rx[u] = Pieces<DT>{};
+      rg[u] = Pieces<DT>{};
+      const long long row = xr + (long long)h * sd.x_h, grow = gr + (long long)h * sd.dy_h;
+      if (h < h_end && plan.on && qchk_span(BS_ROT_IN, row + plan.o0, 4, sd.lim_x) &&
+          qchk_span(BS_ROT_IN, row + plan.o1, 4, sd.lim_x) && qchk_span(BS_ROT_IN, grow + plan.o0, 4, sd.lim_dy) &&
+          qchk_span(BS_ROT_IN, grow + plan.o1, 4, sd.lim_dy)) {
+        rx[u] = load_pieces<DT, kInter>(sd.x, row, plan.o0, plan.o1);
+        rg[u] = load_pieces<DT, kInter>(sd.dy, grow, plan.o0, plan.o1);
+      }
+    }
+  };
+  if (item < items) {
+    begin_item();
+    load();
+  }
+  while (item < items) {
+    Pieces<DT> cx[kUnroll], cg[kUnroll];
     float c[4], s[4];
-    load_turn(p, b * p.table_b + l * p.pairs, plan.pair0, c, s);
-    const long long xr = b * sd.x_b + l * sd.x_l, yr = b * sd.y_b + l * sd.y_l, gr = b * sd.dy_b + l * sd.dy_l;
-    const int h_end = min(sd.heads, (chunk + 1) * p.heads_per_warp);
-    Pieces<DT> rx[kUnroll], rg[kUnroll];
-    auto load = [&](int h0) {
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int h = h0 + u * R + lane / G;
-        rx[u] = Pieces<DT>{};
-        rg[u] = Pieces<DT>{};
-        const long long row = xr + (long long)h * sd.x_h, grow = gr + (long long)h * sd.dy_h;
-        if (h < h_end && plan.on && qchk_span(BS_ROT_IN, row + plan.o0, 4, sd.lim_x) &&
-            qchk_span(BS_ROT_IN, row + plan.o1, 4, sd.lim_x) &&
-            qchk_span(BS_ROT_IN, grow + plan.o0, 4, sd.lim_dy) && qchk_span(BS_ROT_IN, grow + plan.o1, 4, sd.lim_dy)) {
-          rx[u] = load_pieces<DT, kInter>(sd.x, row, plan.o0, plan.o1);
-          rg[u] = load_pieces<DT, kInter>(sd.dy, grow, plan.o0, plan.o1);
-        }
+    for (int u = 0; u < kUnroll; ++u) {
+      cx[u] = rx[u];
+      cg[u] = rg[u];
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      c[i] = c_next[i];
+      s[i] = s_next[i];
+    }
+    const long long to = yr;
+    const int h_now = h0, h_stop = h_end;
+    h0 += R * kUnroll;
+    if (h0 >= h_end) {
+      item += stride;
+      if (item < items) begin_item();
+    }
+    if (item < items) load();
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      if (h_now + u * R >= h_stop) break;
+      const int h = h_now + u * R + lane / G;
+      float x[8], g[8], ss = 0.f, dot = 0.f;
+      pieces_to_float<DT>(cx[u], x);
+      pieces_to_float<DT>(cg[u], g);
+      rotate4<kInter, true>(g, c, s);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        ss = fmaf(x[j], x[j], ss);
+        dot = fmaf(g[j] * w[j], x[j], dot);
       }
-    };
-    const int h_begin = chunk * p.heads_per_warp;
-    load(h_begin);
-    for (int h0 = h_begin; h0 < h_end; h0 += R * kUnroll) {
-      Pieces<DT> cx[kUnroll], cg[kUnroll];  // the next rows' loads are in flight during these rows' arithmetic
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        cx[u] = rx[u];
-        cg[u] = rg[u];
-      }
-      if (h0 + R * kUnroll < h_end) load(h0 + R * kUnroll);
-#pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int h = h0 + u * R + lane / G;
-        float x[8], g[8], ss = 0.f, dot = 0.f;
-        pieces_to_float<DT>(cx[u], x);
-        pieces_to_float<DT>(cg[u], g);
-        rotate4<kInter, true>(g, c, s);
+      ss = group_sum<G>(ss);
+      dot = group_sum<G>(dot);
+      const float rstd = rsqrtf(ss * inv_d + p.eps);
+      const float pull = rstd * rstd * (dot * inv_d);
+      if (h < h_stop) {
+        float o[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          ss = fmaf(x[j], x[j], ss);
-          dot = fmaf(g[j] * w[j], x[j], dot);
+          dw[j] = fmaf(g[j], x[j] * rstd, dw[j]);
+          o[j] = rstd * (g[j] * w[j] - x[j] * pull);
         }
-        ss = group_sum<G>(ss);
-        dot = group_sum<G>(dot);
-        const float rstd = rsqrtf(ss * inv_d + p.eps);
-        const float pull = rstd * rstd * (dot * inv_d);
-        if (h < h_end) {
-          float o[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            dw[j] = fmaf(g[j], x[j] * rstd, dw[j]);
-            o[j] = rstd * (g[j] * w[j] - x[j] * pull);
-          }
-          const long long row = yr + (long long)h * sd.y_h;
-          if (plan.on && qchk_span(BS_ROT_OUT, row + plan.o0, 4, sd.lim_y) &&
-              qchk_span(BS_ROT_OUT, row + plan.o1, 4, sd.lim_y))
-            store_pieces<DT, kInter>(sd.y, row, plan.o0, plan.o1, o);
-        }
+        const long long row = to + (long long)h * sd.y_h;
+        if (plan.on && qchk_span(BS_ROT_OUT, row + plan.o0, 4, sd.lim_y) &&
+            qchk_span(BS_ROT_OUT, row + plan.o1, 4, sd.lim_y))
+          store_pieces<DT, kInter>(sd.y, row, plan.o0, plan.o1, o);
       }
     }
   }
@@ -640,6 +664,8 @@ static void launch_table(const void* positions, int pos_dtype, long long tokens,
 }
 
 constexpr int kMaxHeadDim = 1024;
+// Rows a backward CTA should have at least: each of its partial rows costs D values of traffic again.
+constexpr int kBwdRowsPerCta = 64;
 
 // The vector kernels take heads of whole 8-value pieces up to 256, rotated parts of whole pieces, and rows
 // that start on the pieces' alignment.
@@ -657,15 +683,18 @@ static int lanes_per_row(int D) {
   return g;
 }
 
-// Backward: the CTAs of both sides together, each with a partial row of dw.  Four resident CTAs on each SM
-// or fewer where there are fewer rows.
-static void plan_bwd(long long tokens, int hq, int hk, int rows_per_cta, int (&ctas)[2]) {
-  const long long most = (long long)kBwdCtas * sm_count();
-  const long long rows = tokens * (hq + hk);
-  const long long want = std::max<long long>(2, std::min<long long>(most, rows / rows_per_cta));
-  const int heads[2] = {hq, hk};
+// Backward: the CTAs of both sides together, each with a partial row of dw: as many as are resident at once, or
+// fewer where there are fewer rows.
+static long long bwd_ctas(long long rows) {
+  return std::max<long long>(2, std::min<long long>((long long)kBwdCtas * sm_count(), rows / kBwdRowsPerCta));
+}
+// The sides' shares go by their steps (rows_per_step rows of one token each), not by their rows: two heads take a
+// warp as long as six.
+static void split_bwd(long long rows, int hq, int hk, int rows_per_step, int (&ctas)[2]) {
+  const long long want = bwd_ctas(rows);
+  const long long steps[2] = {(hq + rows_per_step - 1) / rows_per_step, (hk + rows_per_step - 1) / rows_per_step};
   for (int i = 0; i < 2; ++i)
-    ctas[i] = heads[i] == 0 ? 0 : (int)std::max<long long>(1, want * heads[i] / (hq + hk));
+    ctas[i] = steps[i] == 0 ? 0 : (int)std::max<long long>(1, want * steps[i] / (steps[0] + steps[1]));
 }
 
 template <int DT, bool kInter>
@@ -700,13 +729,9 @@ static long long reach(long long n0, long long s0, long long n1, long long s1, l
   return (n0 - 1) * s0 + (n1 - 1) * s1 + (n2 - 1) * s2 + d;
 }
 
-// Rows a backward CTA should have at least: each of its partial rows costs D values of traffic again.
-constexpr int kBwdRowsPerCta = 64;
-
+// split_bwd gives each side at least one CTA: at most one more than bwd_ctas in all.
 static size_t bwd_workspace(long long tokens, int hq, int hk, int D) {
-  int ctas[2];
-  plan_bwd(tokens, hq, hk, kBwdRowsPerCta, ctas);
-  return (size_t)(ctas[0] + ctas[1]) * D * 4;
+  return (size_t)(bwd_ctas(tokens * (hq + hk)) + 1) * D * 4;
 }
 
 struct HeadCall {
@@ -805,7 +830,7 @@ static int head_norm(const HeadCall& a, int dtype, int64_t batch, int64_t tokens
       set_error("%s: workspace too small: need %zu bytes", a.what, need);
       return QLIN_EINVAL;
     }
-    plan_bwd(rows, hq, hk, kBwdRowsPerCta, p.ctas);
+    split_bwd(rows * (hq + hk), hq, hk, vec ? std::max(1, 32 / lanes_per_row(dim)) * bwd_unroll(dtype) : 1, p.ctas);
     if (a.dqw != nullptr) p.side[0].dw = reinterpret_cast<float*>(workspace);
     if (a.dkw != nullptr) p.side[1].dw = reinterpret_cast<float*>(workspace) + (size_t)p.ctas[0] * dim;
     grid = dim3((unsigned)(p.ctas[0] + p.ctas[1]));
