@@ -117,6 +117,9 @@ __global__ void __launch_bounds__(256) rotary_table_kernel(const __grid_constant
 // ---------------------------------------------------------------------------------------------
 // Head norm with rotation
 // ---------------------------------------------------------------------------------------------
+struct HeadParams;
+__device__ __forceinline__ void put_dw(const HeadParams& p, int which, int cta, int i, float sum);
+
 // One of q and k: [B, L, heads, D] with element strides, values of a row side by side.
 struct HeadSide {
   const void* x;
@@ -124,6 +127,7 @@ struct HeadSide {
   void* y;             // forward: the output; backward: dx
   const void* w;       // [D] or null
   float* dw;           // backward: partial sums [ctas][D]
+  void* dw_out;        // backward: the gradient itself, where one CTA has all of the side's rows
   int heads, chunks;   // chunks: warps that share a token's heads
   long long x_b, x_l, x_h, y_b, y_l, y_h, dy_b, dy_l, dy_h;
   long long lim_x, lim_y, lim_dy;  // element counts for the QLIN_CHECKS build
@@ -303,6 +307,20 @@ __device__ __forceinline__ void load_weight(const void* w, int dt, const Plan& p
   } else {
     pieces_to_float<QLIN_BF16>(load_pieces<QLIN_BF16, false>(w, 0, plan.o0, plan.o1), f);
   }
+}
+
+// Column i of a CTA's sum of g * xhat: to its partial row, or rounded once to the gradient.
+__device__ __forceinline__ void put_dw(const HeadParams& p, int which, int cta, int i, float sum) {
+  const HeadSide& sd = p.side[which];
+  if (sd.dw_out != nullptr) {
+    if (!qchk(BS_ROT_OUT, i, p.D)) return;
+    if (p.w_dtype == QLIN_F16) head_store<QLIN_F16>(sd.dw_out, i, sum);
+    else if (p.w_dtype == QLIN_BF16) head_store<QLIN_BF16>(sd.dw_out, i, sum);
+    else head_store<QLIN_F32>(sd.dw_out, i, sum);
+    return;
+  }
+  const long long at = (long long)cta * p.D + i;
+  if (qchk(BS_ROT_OUT, at, (long long)p.ctas[which] * p.D)) sd.dw[at] = sum;
 }
 
 // Batch and position of a token.
@@ -489,7 +507,7 @@ __global__ void __launch_bounds__(256, kBwdCtas) qk_norm_rotary_bwd_kernel(const
       }
     }
   }
-  if (sd.dw == nullptr) return;
+  if (sd.dw == nullptr && sd.dw_out == nullptr) return;
 #pragma unroll
   for (int j = 0; j < 8; ++j)
     if (plan.on) part[warp * R + lane / G][(j < 4 ? plan.o0 : plan.o1 - 4) + j] = dw[j];
@@ -498,8 +516,7 @@ __global__ void __launch_bounds__(256, kBwdCtas) qk_norm_rotary_bwd_kernel(const
     float sum = 0.f;
 #pragma unroll
     for (int r = 0; r < 8 * R; ++r) sum += part[r][i];
-    const long long at = (long long)cta * p.D + i;
-    if (qchk(BS_ROT_OUT, at, (long long)p.ctas[which] * p.D)) sd.dw[at] = sum;
+    put_dw(p, which, cta, i, sum);
   }
 }
 
@@ -617,13 +634,12 @@ __global__ void __launch_bounds__(256) qk_norm_rotary_any_kernel(const __grid_co
     }
   }
   if constexpr (kBack) {
-    if (sd.dw == nullptr) return;
+    if (sd.dw == nullptr && sd.dw_out == nullptr) return;
     __syncthreads();
     for (int i = threadIdx.x; i < p.D; i += 256) {
       float sum = 0.f;
       for (int r = 0; r < 8; ++r) sum += warp_dw[r * p.D + i];
-      const long long at = (long long)cta * p.D + i;
-      if (qchk(BS_ROT_OUT, at, (long long)p.ctas[which] * p.D)) sd.dw[at] = sum;
+      put_dw(p, which, cta, i, sum);
     }
   }
 }
@@ -665,7 +681,7 @@ static void launch_table(const void* positions, int pos_dtype, long long tokens,
 
 constexpr int kMaxHeadDim = 1024;
 // Rows a backward CTA should have at least: each of its partial rows costs D values of traffic again.
-constexpr int kBwdRowsPerCta = 64;
+constexpr int kBwdRowsPerCta = 32;
 
 // The vector kernels take heads of whole 8-value pieces up to 256, rotated parts of whole pieces, and rows
 // that start on the pieces' alignment.
@@ -815,7 +831,7 @@ static int head_norm(const HeadCall& a, int dtype, int64_t batch, int64_t tokens
   }
   // A warp's share of a token's heads: all of q or of k where there are tokens enough to fill the machine
   // (about 32 warps on each SM), else as few as one set of unrolled rows.
-  const int step = std::max(1, 32 / lanes_per_row(dim)) * 2;
+  const int step = std::max(1, 32 / lanes_per_row(dim)) * (a.back ? bwd_unroll(dtype) : 2);
   int per_warp = std::max(hq, hk);
   const long long warps = 32ll * sm_count();
   const int fewest = (std::max(hq, hk) + 16383) / 16384;  // the shares are a grid dimension
@@ -831,8 +847,13 @@ static int head_norm(const HeadCall& a, int dtype, int64_t batch, int64_t tokens
       return QLIN_EINVAL;
     }
     split_bwd(rows * (hq + hk), hq, hk, vec ? std::max(1, 32 / lanes_per_row(dim)) * bwd_unroll(dtype) : 1, p.ctas);
-    if (a.dqw != nullptr) p.side[0].dw = reinterpret_cast<float*>(workspace);
-    if (a.dkw != nullptr) p.side[1].dw = reinterpret_cast<float*>(workspace) + (size_t)p.ctas[0] * dim;
+    if (p.ctas[0] <= 1 && p.ctas[1] <= 1) {  // few rows: no partial sums, one launch
+      p.side[0].dw_out = hq > 0 ? a.dqw : nullptr;
+      p.side[1].dw_out = hk > 0 ? a.dkw : nullptr;
+    } else {
+      if (a.dqw != nullptr) p.side[0].dw = reinterpret_cast<float*>(workspace);
+      if (a.dkw != nullptr) p.side[1].dw = reinterpret_cast<float*>(workspace) + (size_t)p.ctas[0] * dim;
+    }
     grid = dim3((unsigned)(p.ctas[0] + p.ctas[1]));
   } else if (vec) {
     if ((rows + 7) / 8 > 0x7fffffff) {
@@ -850,13 +871,16 @@ static int head_norm(const HeadCall& a, int dtype, int64_t batch, int64_t tokens
   else launch_dtype<QLIN_F32>(p, vec, a.back, grid, stream);
   int rc = rot_launched(a.what);
   if (rc || !a.back || (a.dqw == nullptr && a.dkw == nullptr)) return rc;
+  // What is left: a side's partial rows to add up, or a side without heads, whose gradient is zeros.
+  const bool direct = p.ctas[0] <= 1 && p.ctas[1] <= 1;
+  if (direct && (hq > 0 || a.dqw == nullptr) && (hk > 0 || a.dkw == nullptr)) return rc;
   DwParams d{};
   d.part[0] = p.side[0].dw;
   d.part[1] = p.side[1].dw;
   d.ctas[0] = p.ctas[0];
   d.ctas[1] = p.ctas[1];
-  d.out[0] = a.dqw;
-  d.out[1] = a.dkw;
+  d.out[0] = direct && hq > 0 ? nullptr : a.dqw;
+  d.out[1] = direct && hk > 0 ? nullptr : a.dkw;
   d.D = dim;
   d.w_dtype = w_dtype;
   cudaLaunchConfig_t cfg = {};
