@@ -12,8 +12,8 @@
 // each token's scale comes from shared memory.
 //
 // Warp roles (384 threads, one tile to a CTA):
-//   warp 0       weight stream (TMA)       warp 1   TMEM alloc + MMA issuer       (warps 2, 3 idle)
-//   warps 4..7   quantizers                warps 8..11   rescale, join, output
+//   warp 0       weight stream (TMA)       warp 1   TMEM alloc + MMA issuer
+//   warps 2..7   quantizers                warps 8..11   rescale, join, output
 #pragma once
 #include <cuda.h>
 
@@ -186,11 +186,11 @@ fp8_small_kernel(const __grid_constant__ CUtensorMap tmap_w, const Fp8SmallParam
         if (globaltimer() - t0 > QLIN_WAIT_TIMEOUT_NS) break;
       }
     }
-  } else if (warp >= 4 && warp < 8) {
+  } else if (warp < 8) {
     // --------------------------------------------------------------------- quantizers
-    // A warp takes every fourth block, 8 tokens of it at a time, 16 lanes to a token's block; the next 8
+    // A warp takes every sixth block, 8 tokens of it at a time, 16 lanes to a token's block; the next 8
     // tokens' values (of this or of its next block) are in flight meanwhile.
-    constexpr int kPairs = 4;
+    constexpr int kPairs = 4, kWarps = 6;
     const int groups = (min(p.M, TN) + 7) / 8;
     const int col = (lane & 15) * 8;
     Raw8<DT> raw[kPairs];
@@ -200,8 +200,8 @@ fp8_small_kernel(const __grid_constant__ CUtensorMap tmap_w, const Fp8SmallParam
         raw[u] = small_load8<DT>(p, g * 8 + u * 2 + (lane >> 4), (b_begin + i) * 128 + col);
     };
     bool ok = true;
-    if (warp - 4 < blocks) load(warp - 4, 0);
-    for (int i = warp - 4; i < blocks && ok; i += 4) {
+    if (warp - 2 < blocks) load(warp - 2, 0);
+    for (int i = warp - 2; i < blocks && ok; i += kWarps) {
       const int s = i % R;
       uint8_t* tile = sx + s * Cfg::kXStage;
       for (int g = 0; g < groups; ++g) {
@@ -213,7 +213,7 @@ fp8_small_kernel(const __grid_constant__ CUtensorMap tmap_w, const Fp8SmallParam
           a[u] = max(kAmaxFloorBits, raw8_amax_bits<DT>(now[u]));
         }
         if (g + 1 < groups) load(i, g + 1);
-        else if (i + 4 < blocks) load(i + 4, 0);
+        else if (i + kWarps < blocks) load(i + kWarps, 0);
         // each lane ends up with the maximum of pair (lane >> 2) & 3 of its half, as in the row quantizer
 #pragma unroll
         for (int o = 8, n = 2; o > 2; o >>= 1, n >>= 1) {
@@ -254,7 +254,7 @@ fp8_small_kernel(const __grid_constant__ CUtensorMap tmap_w, const Fp8SmallParam
       __syncwarp();
       if (lane == 0) mbar_arrive(&x_full[s]);
     }
-  } else if (warp >= 8) {
+  } else {
     // --------------------------------------------------------------------- rescale
     const int quarter = warp & 3;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
