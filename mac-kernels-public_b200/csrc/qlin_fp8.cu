@@ -56,7 +56,7 @@ __device__ __forceinline__ uint4 aligned_word(const uint8_t* at, int w, const ui
 }
 
 template <int DT, bool kVec>
-__global__ void __launch_bounds__(256) quant_rows_fp8_kernel(const QuantFp8Params p) {
+__global__ void __launch_bounds__(256, DT == QLIN_F32 ? 2 : 4) quant_rows_fp8_kernel(const QuantFp8Params p) {
   constexpr int kRows = 8;
   griddep_launch();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(256) quant_rows_fp8_kernel(const QuantFp8Param
   if (m0 >= p.M) return;
   const int c = b * 128 + (lane & 15) * 8;
   const int rows = min(kRows, p.M - m0);
-  float f[kRows][8];
+  Raw8<DT> raw[kRows];  // kept as stored: as fp32 they would take twice the registers
   if constexpr (!kVec) {
     // Rows that start off a 16-byte boundary: every lane reads the aligned words its values begin in, and takes
     // what they end in from the next lane; the words after the last lane's are read by a lane for each row.
@@ -106,39 +106,24 @@ __global__ void __launch_bounds__(256) quant_rows_fp8_kernel(const QuantFp8Param
       last.z = __shfl_sync(0xffffffffu, past.z, i);
       last.w = __shfl_sync(0xffffffffu, past.w, i);
       a.v[kOwn] = lane == 31 ? last : next;
-      raw8_to_float<DT>(a.values(), f[i]);
-      if (c + 8 > p.K) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) f[i][j] = c + j < p.K ? f[i][j] : 0.f;
-      }
+      raw[i] = a.values();
+      if (c + 8 > p.K) raw[i] = raw8_first<DT>(raw[i], p.K - c);
     }
-  } else if (c + 8 <= p.K) {
-    Raw8<DT> raw[kRows];
+  } else {
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
       const long long at = (long long)(m0 + min(i, rows - 1)) * p.ldx + c;
       raw[i] = Raw8<DT>{};
-      if (qchk_span(BS_FP8_QUANT, at, 8, p.lim_x)) raw[i] = load_raw8<DT>(p.x, at);
+      if (c < p.K && qchk_span(BS_FP8_QUANT, at, min(8, p.K - c), p.lim_x))
+        raw[i] = c + 8 <= p.K ? load_raw8<DT>(p.x, at) : gather_raw8<DT>(p.x, at, p.K - c);
     }
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) raw8_to_float<DT>(raw[i], f[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < kRows; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const long long at = (long long)(m0 + i) * p.ldx + c + j;
-        f[i][j] = (i < rows && c + j < p.K && qchk(BS_FP8_QUANT, at, p.lim_x)) ? load_elem<DT>(p.x, at) : 0.f;
-      }
   }
   // Each of the 16 lanes ends up with the maximum of one of the 8 rows (two lanes to a row): at every
   // step a lane hands the half of its rows to its partner that it does not keep.
   uint32_t a[kRows];
 #pragma unroll
   for (int i = 0; i < kRows; ++i) {
-    a[i] = kAmaxFloorBits;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) a[i] = max(a[i], __float_as_uint(f[i][j]) & 0x7fffffffu);
+    a[i] = max(kAmaxFloorBits, raw8_amax_bits<DT>(raw[i]));
   }
 #pragma unroll
   for (int o = 8, n = 4; o > 1; o >>= 1, n >>= 1) {
@@ -157,9 +142,11 @@ __global__ void __launch_bounds__(256) quant_rows_fp8_kernel(const QuantFp8Param
     const float r = __shfl_sync(0xffffffffu, up, (lane & 16) | (i << 1));
     if (i < rows && b < p.kb) {
       const long long at = (long long)(m0 + i) * p.ldq + c;
+      float f[8];
+      raw8_to_float<DT>(raw[i], f);
       if (qchk_span(BS_FP8_QUANT, at, 8, p.lim_q))
-        *reinterpret_cast<uint2*>(p.q + at) = make_uint2(to_e4m3x4(f[i][0], f[i][1], f[i][2], f[i][3], r),
-                                                         to_e4m3x4(f[i][4], f[i][5], f[i][6], f[i][7], r));
+        *reinterpret_cast<uint2*>(p.q + at) = make_uint2(to_e4m3x4(f[0], f[1], f[2], f[3], r),
+                                                         to_e4m3x4(f[4], f[5], f[6], f[7], r));
     }
   }
   const int row = (lane >> 1) & 7;

@@ -11,13 +11,6 @@ namespace qlin {
 constexpr float kE4m3Max = 448.f;
 constexpr uint32_t kAmaxFloorBits = (127 - 100) << 23;  // 2^-100
 
-template <int DT>
-__device__ __forceinline__ float load_elem(const void* x, long long i) {
-  if constexpr (DT == QLIN_F16) return __half2float(reinterpret_cast<const __half*>(x)[i]);
-  else if constexpr (DT == QLIN_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(x)[i]);
-  else return reinterpret_cast<const float*>(x)[i];
-}
-
 // 8 consecutive values as stored: 16 bytes of a 2-byte type, 32 of fp32.
 template <int DT>
 struct Raw8 {
@@ -126,6 +119,42 @@ __device__ __forceinline__ void raw8_to_float(const Raw8<DT>& r, float (&f)[8]) 
     f[6] = __uint_as_float(r.v[1].z);
     f[7] = __uint_as_float(r.v[1].w);
   }
+}
+
+// The same with the values from the n-th on set to zero.
+template <int DT>
+__device__ __forceinline__ Raw8<DT> raw8_first(Raw8<DT> r, int n) {
+  uint32_t w[DT == QLIN_F32 ? 8 : 4] = {r.v[0].x, r.v[0].y, r.v[0].z, r.v[0].w};
+  if constexpr (DT == QLIN_F32) {
+    w[4] = r.v[1].x;
+    w[5] = r.v[1].y;
+    w[6] = r.v[1].z;
+    w[7] = r.v[1].w;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = j < n ? w[j] : 0;
+    r.v[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = 2 * j + 1 < n ? w[j] : 2 * j < n ? w[j] & 0xffffu : 0;
+  }
+  r.v[0] = make_uint4(w[0], w[1], w[2], w[3]);
+  return r;
+}
+
+// n of 8 consecutive values, one by one, and zeros.
+template <int DT>
+__device__ __forceinline__ Raw8<DT> gather_raw8(const void* x, long long i, int n) {
+  uint32_t w[DT == QLIN_F32 ? 8 : 4] = {};
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if (j >= n) continue;
+    if constexpr (DT == QLIN_F32) w[j] = reinterpret_cast<const uint32_t*>(x)[i + j];
+    else w[j / 2] |= (uint32_t) reinterpret_cast<const uint16_t*>(x)[i + j] << (16 * (j & 1));
+  }
+  Raw8<DT> r;
+  r.v[0] = make_uint4(w[0], w[1], w[2], w[3]);
+  if constexpr (DT == QLIN_F32) r.v[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  return r;
 }
 
 // Bit pattern, as fp32, of the largest magnitude among the 8.  Patterns of one type order like the

@@ -65,16 +65,7 @@ __device__ __forceinline__ Raw8<DT> small_load8(const Fp8SmallParams& p, int m, 
       raw = p.x_vec ? load_raw8<DT>(p.x, at) : load_raw8_any<DT>(p.x, at, p.lim_x);
     return raw;
   }
-  uint32_t w[DT == QLIN_F32 ? 8 : 4] = {};
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    if (c + j >= p.K || !qchk(BS_FP8_X, at + j, p.lim_x)) continue;
-    if constexpr (DT == QLIN_F32) w[j] = reinterpret_cast<const uint32_t*>(p.x)[at + j];
-    else w[j / 2] |= (uint32_t) reinterpret_cast<const uint16_t*>(p.x)[at + j] << (16 * (j & 1));
-  }
-  raw.v[0] = make_uint4(w[0], w[1], w[2], w[3]);
-  if constexpr (DT == QLIN_F32) raw.v[1] = make_uint4(w[4], w[5], w[6], w[7]);
-  return raw;
+  return qchk_span(BS_FP8_X, at, p.K - c, p.lim_x) ? gather_raw8<DT>(p.x, at, p.K - c) : raw;
 }
 
 __device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {

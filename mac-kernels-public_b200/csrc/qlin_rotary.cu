@@ -45,8 +45,11 @@ __device__ __forceinline__ unsigned long long turns_of(long long pos, unsigned l
 __device__ __forceinline__ unsigned long long turns_of(float pos, unsigned long long turn) {
   const uint32_t bits = __float_as_uint(pos);
   const int e = max((int)((bits >> 23) & 255), 1) - 150;  // pos = +- mantissa * 2^e
-  const unsigned long long mant = (bits & 0x7fffff) | ((bits & 0x7f800000) ? 0x800000 : 0);
-  const unsigned long long lo = mant * turn, hi = __umul64hi(mant, turn);
+  const uint32_t mant = (bits & 0x7fffff) | ((bits & 0x7f800000) ? 0x800000 : 0);
+  // the 88-bit product, by the turn's halves
+  const unsigned long long p0 = (unsigned long long)mant * (uint32_t)turn;
+  const unsigned long long p1 = (unsigned long long)mant * (uint32_t)(turn >> 32);
+  const unsigned long long lo = (p1 << 32) + p0, hi = (p1 + (p0 >> 32)) >> 32;
   unsigned long long u;
   if (e >= 0) u = e < 64 ? lo << e : 0;
   else if (e > -64) u = (lo >> -e) | (hi << (64 + e));
@@ -77,8 +80,9 @@ __device__ __forceinline__ float2 cos_sin_of(unsigned long long u) {
 
 // The angle is kept in turns as a 64-bit fraction until its whole turns are gone, so large positions lose
 // nothing.  A thread keeps its pair's frequency and walks over tokens, four at a time; a warp writes 256
-// consecutive bytes.  Measured at 32760 tokens of 64 pairs against the same sum in fp64 and sincospif:
-// NEW us against 12.6 us (the fp64 pipe and the conversions bound that one).
+// consecutive bytes.  Bound by instructions.  Measured at 32760 tokens of 64 pairs (16.8 MB written): 6.5 us from
+// int64 positions, 9.7 us from fp32 ones; with the frequencies read through the constant cache, one lane's entry at a
+// time, 14 us; with 8 CTAs on each SM and 64-bit divisions instead of walking pointers, 8.6 us.
 template <int CAP, typename POS>
 __global__ void __launch_bounds__(256) rotary_table_kernel(const __grid_constant__ RotTableParams<CAP> p) {
   const int pair = blockIdx.y * 32 + threadIdx.x;
@@ -90,18 +94,19 @@ __global__ void __launch_bounds__(256) rotary_table_kernel(const __grid_constant
   const int axis = params->axis[pair];
   const POS* pos = reinterpret_cast<const POS*>(p.pos);
   constexpr int kTokens = 4;
-  const long long step = (long long)gridDim.x * 8;
-  for (long long t0 = (long long)blockIdx.x * 8 + threadIdx.y; t0 < p.tokens; t0 += step * kTokens) {
+  const long long step = (long long)gridDim.x * 8, first = (long long)blockIdx.x * 8 + threadIdx.y;
+  const POS* from = pos + first * p.axes + axis;
+  float2* to = p.out + first * p.pairs + pair;
+  const long long from_step = step * p.axes, to_step = step * p.pairs;
+  for (long long left = p.tokens - first; left > 0; left -= kTokens * step) {
     POS x[kTokens];
 #pragma unroll
     for (int u = 0; u < kTokens; ++u) {
-      const long long at = (t0 + u * step) * p.axes + axis;
-      x[u] = (t0 + u * step < p.tokens && qchk(BS_ROT_IN, at, p.tokens * p.axes)) ? __ldg(pos + at) : POS(0);
+      x[u] = (u * step < left && qchk(BS_ROT_IN, from - pos, p.tokens * p.axes)) ? __ldg(from) : POS(0);
+      from += from_step;
     }
 #pragma unroll
     for (int u = 0; u < kTokens; ++u) {
-      const long long at = (t0 + u * step) * p.pairs + pair;
-      if (t0 + u * step >= p.tokens || !qchk(BS_ROT_OUT, at, p.tokens * p.pairs)) continue;
       float2 v;
       if constexpr (std::is_same<POS, float>::value) {
         v = cos_sin_of(turns_of(x[u], turn));
@@ -109,7 +114,8 @@ __global__ void __launch_bounds__(256) rotary_table_kernel(const __grid_constant
       } else {
         v = cos_sin_of(turns_of((long long)x[u], turn));
       }
-      p.out[at] = v;
+      if (u * step < left && qchk(BS_ROT_OUT, to - p.out, p.tokens * p.pairs)) *to = v;
+      to += to_step;
     }
   }
 }
@@ -673,7 +679,7 @@ static void launch_table(const void* positions, int pos_dtype, long long tokens,
       p.axis[at] = (unsigned char)a;
     }
   }
-  const dim3 block(32, 8), grid((unsigned)std::min<long long>((tokens + 7) / 8, 8ll * sm_count()), (pairs + 31) / 32);
+  const dim3 block(32, 8), grid((unsigned)std::min<long long>((tokens + 7) / 8, 2ll * sm_count()), (pairs + 31) / 32);
   if (pos_dtype == QLIN_F32) rotary_table_kernel<CAP, float><<<grid, block, 0, s>>>(p);
   else if (pos_dtype == QLIN_I32) rotary_table_kernel<CAP, int><<<grid, block, 0, s>>>(p);
   else rotary_table_kernel<CAP, long long><<<grid, block, 0, s>>>(p);
