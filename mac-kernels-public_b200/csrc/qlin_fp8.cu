@@ -59,6 +59,7 @@ template <int DT, bool kVec>
 __global__ void __launch_bounds__(256, DT == QLIN_F32 ? 2 : 4) quant_rows_fp8_kernel(const QuantFp8Params p) {
   constexpr int kRows = 8;
   griddep_launch();
+  griddep_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t item = blockIdx.x * 8u + warp;  // a warp takes 8 rows of two blocks; neighbours the next blocks
   const int row_tile = (int)(item / (uint32_t)p.k_pairs);
@@ -179,14 +180,15 @@ static int launch_quant_rows_fp8(const void* x, int x_dtype, long long ldx, int 
   }
   const int esz = x_dtype == QLIN_F32 ? 4 : 2;
   const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (ldx * esz) % 16 == 0;
-#define QLIN_QUANT_FP8(DT)                                                              \
-  if (vec) quant_rows_fp8_kernel<DT, true><<<(unsigned)grid, 256, 0, stream>>>(p);      \
-  else quant_rows_fp8_kernel<DT, false><<<(unsigned)grid, 256, 0, stream>>>(p);
+  const dim3 ctas((unsigned)grid), threads(256);
+  cudaError_t e;
+#define QLIN_QUANT_FP8(DT)                                                                    \
+  e = vec ? launch_dependent(quant_rows_fp8_kernel<DT, true>, ctas, threads, 0, stream, 0, p) \
+          : launch_dependent(quant_rows_fp8_kernel<DT, false>, ctas, threads, 0, stream, 0, p);
   if (x_dtype == QLIN_F16) { QLIN_QUANT_FP8(QLIN_F16) }
   else if (x_dtype == QLIN_BF16) { QLIN_QUANT_FP8(QLIN_BF16) }
   else { QLIN_QUANT_FP8(QLIN_F32) }
 #undef QLIN_QUANT_FP8
-  const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) {
     set_error("fp8 quantizer launch failed: %s", cudaGetErrorString(e));
     return QLIN_ECUDA;
@@ -215,21 +217,8 @@ static int launch_fp8(const CUtensorMap& tx, const CUtensorMap& tw, const CUtens
   }
   const int tiles = p.m_tiles * p.n_tiles;
   const int share = CTAS == 2 ? 2 : p.splits;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(share * std::min(tiles, sm_count() / share)));
-  cfg.blockDim = dim3(Cfg::kThreads);
-  cfg.dynamicSmemBytes = Cfg::kSmem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)share;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // set up while the quantizer runs
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = p.kb > 0 ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tx, tw, ty, p);
+  const cudaError_t e = launch_dependent(kern, dim3((unsigned)(share * std::min(tiles, sm_count() / share))),
+                                         dim3(Cfg::kThreads), Cfg::kSmem, stream, (unsigned)share, tx, tw, ty, p);
   if (e != cudaSuccess) {
     set_error("fp8 gemm launch failed: %s", cudaGetErrorString(e));
     return QLIN_ECUDA;
@@ -257,19 +246,8 @@ static int launch_fp8_small(const CUtensorMap& tw, const Fp8SmallParams& p, cuda
   const int at_once = sm_count() * Cfg::kCtas;
   int splits = 1;
   while (splits < 8 && splits * 2 * 3 <= p.kb && tiles * splits * 2 <= at_once) splits *= 2;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(tiles * splits));
-  cfg.blockDim = dim3(Cfg::kThreads);
-  cfg.dynamicSmemBytes = Cfg::kSmem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)splits;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tw, p, splits);
+  const cudaError_t e = launch_dependent(kern, dim3((unsigned)(tiles * splits)), dim3(Cfg::kThreads), Cfg::kSmem, stream,
+                                         (unsigned)splits, tw, p, splits);
   if (e != cudaSuccess) {
     set_error("fp8 small-M launch failed: %s", cudaGetErrorString(e));
     return QLIN_ECUDA;
@@ -383,7 +361,6 @@ static int fp8_product(const char* what, const void* x, int x_dtype, int64_t m, 
   if (m <= kSmallM && kb > 0) {
     Fp8SmallParams p{};
     p.x = x;
-    p.x_dtype = x_dtype;
     p.x_vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0 && (m == 1 || (ldx * (x_dtype == QLIN_F32 ? 4 : 2)) % 16 == 0);
     p.ldx = ldx;
     p.M = (int)m;

@@ -61,11 +61,6 @@ struct Around8 {
       for (int j = 0; j < kWords / 4; ++j) v[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
     }
   }
-  __device__ __forceinline__ void clear() {
-    off = 16;
-#pragma unroll
-    for (int j = 0; j < kWords / 4; ++j) v[j] = uint4{};
-  }
   __device__ __forceinline__ Raw8<DT> values() const {
     uint32_t w[kWords + 1];
 #pragma unroll

@@ -24,7 +24,6 @@ namespace qlin {
 
 struct Fp8SmallParams {
   const void* x;
-  int x_dtype;
   int x_vec;        // rows of x take 16-byte loads
   long long ldx;
   int M, N, K;      // tokens, output channels, contraction
@@ -127,6 +126,8 @@ fp8_small_kernel(const __grid_constant__ CUtensorMap tmap_w, const Fp8SmallParam
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  griddep_launch();
+  griddep_wait();
   float acc[TN];  // rescale warps: this channel's sums, a token each
 
   if (warp == 0) {

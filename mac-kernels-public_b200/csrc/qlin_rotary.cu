@@ -85,6 +85,7 @@ __device__ __forceinline__ float2 cos_sin_of(unsigned long long u) {
 // time, 14 us; with 8 CTAs on each SM and 64-bit divisions instead of walking pointers, 8.6 us.
 template <int CAP, typename POS>
 __global__ void __launch_bounds__(256) rotary_table_kernel(const __grid_constant__ RotTableParams<CAP> p) {
+  griddep_launch();
   const int pair = blockIdx.y * 32 + threadIdx.x;
   if (pair >= p.pairs) return;
   // Read by address, as ordinary memory: the constant cache serves one lane's entry at a time.
@@ -94,6 +95,7 @@ __global__ void __launch_bounds__(256) rotary_table_kernel(const __grid_constant
   const int axis = params->axis[pair];
   const POS* pos = reinterpret_cast<const POS*>(p.pos);
   constexpr int kTokens = 4;
+  griddep_wait();
   const long long step = (long long)gridDim.x * 8, first = (long long)blockIdx.x * 8 + threadIdx.y;
   const POS* from = pos + first * p.axes + axis;
   float2* to = p.out + first * p.pairs + pair;
@@ -355,6 +357,8 @@ template <int DT, int G, bool kInter>
 __global__ void __launch_bounds__(256, 4) qk_norm_rotary_kernel(const __grid_constant__ HeadParams p) {
   constexpr int R = 32 / G;
   constexpr int kUnroll = DT == QLIN_F32 ? 2 : 4;
+  griddep_launch();
+  griddep_wait();
   const int lane = threadIdx.x & 31;
   int chunk = blockIdx.y;
   const int which = chunk >= p.side[0].chunks ? 1 : 0;
@@ -413,6 +417,7 @@ __global__ void __launch_bounds__(256, kBwdCtas) qk_norm_rotary_bwd_kernel(const
   constexpr int kUnroll = bwd_unroll(DT);
   __shared__ float part[8 * R][G * 8];
   griddep_launch();
+  griddep_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int which = blockIdx.x >= (unsigned)p.ctas[0] ? 1 : 0;
   const int cta = which ? blockIdx.x - p.ctas[0] : blockIdx.x;
@@ -536,6 +541,7 @@ struct DwParams {
 // dw = the sum of the partial rows: 32 columns to a CTA, 32 rows at a time, one rounding to the weight's type.
 __global__ void __launch_bounds__(1024) dw_sum_kernel(const DwParams p) {
   __shared__ float part[32][33];
+  griddep_launch();
   griddep_wait();
   const int which = blockIdx.y;
   const int i = blockIdx.x * 32 + threadIdx.x;
@@ -564,7 +570,8 @@ __global__ void __launch_bounds__(1024) dw_sum_kernel(const DwParams p) {
 template <int DT, bool kBack>
 __global__ void __launch_bounds__(256) qk_norm_rotary_any_kernel(const __grid_constant__ HeadParams p) {
   extern __shared__ float warp_dw[];  // backward: [8][D]
-  if constexpr (kBack) griddep_launch();
+  griddep_launch();
+  griddep_wait();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int which = blockIdx.x >= (unsigned)p.ctas[0] ? 1 : 0;
   const int cta = which ? blockIdx.x - p.ctas[0] : blockIdx.x;
@@ -680,9 +687,9 @@ static void launch_table(const void* positions, int pos_dtype, long long tokens,
     }
   }
   const dim3 block(32, 8), grid((unsigned)std::min<long long>((tokens + 7) / 8, 2ll * sm_count()), (pairs + 31) / 32);
-  if (pos_dtype == QLIN_F32) rotary_table_kernel<CAP, float><<<grid, block, 0, s>>>(p);
-  else if (pos_dtype == QLIN_I32) rotary_table_kernel<CAP, int><<<grid, block, 0, s>>>(p);
-  else rotary_table_kernel<CAP, long long><<<grid, block, 0, s>>>(p);
+  if (pos_dtype == QLIN_F32) launch_dependent(rotary_table_kernel<CAP, float>, grid, block, 0, s, 0, p);
+  else if (pos_dtype == QLIN_I32) launch_dependent(rotary_table_kernel<CAP, int>, grid, block, 0, s, 0, p);
+  else launch_dependent(rotary_table_kernel<CAP, long long>, grid, block, 0, s, 0, p);
 }
 
 constexpr int kMaxHeadDim = 1024;
@@ -724,8 +731,8 @@ static void launch_rows(const HeadParams& p, int g, bool back, dim3 grid, cudaSt
   switch (g) {
 #define QLIN_ROWS(G)                                                                    \
   case G:                                                                               \
-    if (back) qk_norm_rotary_bwd_kernel<DT, G, kInter><<<grid, 256, 0, s>>>(p);         \
-    else qk_norm_rotary_kernel<DT, G, kInter><<<grid, 256, 0, s>>>(p);                  \
+    if (back) launch_dependent(qk_norm_rotary_bwd_kernel<DT, G, kInter>, grid, dim3(256), 0, s, 0, p); \
+    else launch_dependent(qk_norm_rotary_kernel<DT, G, kInter>, grid, dim3(256), 0, s, 0, p);          \
     break;
     QLIN_ROWS(4)
     QLIN_ROWS(8)
@@ -738,8 +745,8 @@ static void launch_rows(const HeadParams& p, int g, bool back, dim3 grid, cudaSt
 template <int DT>
 static void launch_dtype(const HeadParams& p, bool vec, bool back, dim3 grid, cudaStream_t s) {
   if (!vec) {
-    if (back) qk_norm_rotary_any_kernel<DT, true><<<grid, 256, (size_t)8 * p.D * 4, s>>>(p);
-    else qk_norm_rotary_any_kernel<DT, false><<<grid, 256, 0, s>>>(p);
+    if (back) launch_dependent(qk_norm_rotary_any_kernel<DT, true>, grid, dim3(256), (size_t)8 * p.D * 4, s, 0, p);
+    else launch_dependent(qk_norm_rotary_any_kernel<DT, false>, grid, dim3(256), 0, s, 0, p);
   } else if (p.interleaved) {
     launch_rows<DT, true>(p, lanes_per_row(p.D), back, grid, s);
   } else {
@@ -889,17 +896,8 @@ static int head_norm(const HeadCall& a, int dtype, int64_t batch, int64_t tokens
   d.out[1] = direct && hk > 0 ? nullptr : a.dkw;
   d.D = dim;
   d.w_dtype = w_dtype;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((dim + 31) / 32, 2);
-  cfg.blockDim = dim3(32, 32);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // set up while the rows are summed
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, dw_sum_kernel, d) != cudaSuccess) return rot_launched(a.what);
-  return QLIN_OK;
+  launch_dependent(dw_sum_kernel, dim3((dim + 31) / 32, 2), dim3(32, 32), 0, stream, 0, d);
+  return rot_launched(a.what);
 }
 
 // This translation unit's bounds record (QLIN_CHECKS build).
