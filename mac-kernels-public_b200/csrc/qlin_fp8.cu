@@ -22,7 +22,9 @@ namespace qlin {
 //
 // One pass over x, bound by HBM: a warp takes 8 rows of two blocks, 16 lanes to a block and 8 values
 // to a lane, with all its loads issued before the first reduction; the 8 scales of a block, which lie
-// side by side in the block-major scale array, go out as one 32-byte piece.
+// side by side in the block-major scale array, go out as one 32-byte piece.  Values stay as they are stored until
+// they are scaled: four CTAs on an SM in 16 bits.  Measured: 4608 x 16384 bf16 in 37 us (6.1 TB/s read and
+// written), 4608 x 6144 in 17; rows off 16-byte boundaries, 7993 x 4565 bf16, 27 us (4.0 TB/s).
 // ---------------------------------------------------------------------------------------------
 struct QuantFp8Params {
   const void* x;

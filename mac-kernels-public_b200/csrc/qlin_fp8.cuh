@@ -12,6 +12,11 @@
 // cores fill the next buffer.  Tokens lie on the TMEM lanes: a thread owns one token, whose scale times
 // the warp's block scale is one factor for all of its values.
 //
+// Measured at 4608 x 6144 x 16384 (bf16): 388 us for this kernel in short bursts (2.4 PFLOP/s, tensor pipe 66%
+// busy), 440 in a long row of calls, where the card's power limit sets the clock to 1.46 GHz.  Without the rescale
+// it takes a fifth less; L2 (36%) and DRAM (8%) wait.  The rescale's own cost is its instructions, about 160 a
+// warp and block, 64 of them packed FMAs; TMEM loads of 16 or 32 columns and one or two in flight take the same.
+//
 // Warp roles (384 threads, one CTA per SM, persistent over the tiles):
 //   warp 0        TMA producer            warp 1   TMEM alloc + MMA issuer       (warps 2, 3 idle)
 //   warps 4..11   rescale + epilogue: two warps per TMEM lane quarter, half the columns each

@@ -352,7 +352,9 @@ __device__ __forceinline__ float group_sum(float v) {
 
 // Forward.  A row is G lanes of 8 values; a warp takes a share of a token's q or k heads (all of them where
 // there are tokens enough), 32 / G rows at a time with kUnroll loads in flight, and keeps the token's cosines
-// and sines in registers, and the weight for all of its tokens.  blockIdx.y is the share.
+// and sines and the weight in registers.  blockIdx.y is the share.  Bound by HBM: 32760 tokens of 80 heads of 128
+// in bf16 take 209 us (6.5 TB/s) with 32 warps on an SM; walking over tokens with fewer CTAs took 217 to 250, more
+// loads ahead at 24 or 16 warps 223 to 250.
 template <int DT, int G, bool kInter>
 __global__ void __launch_bounds__(256, 4) qk_norm_rotary_kernel(const __grid_constant__ HeadParams p) {
   constexpr int R = 32 / G;
@@ -408,7 +410,10 @@ __global__ void __launch_bounds__(256, 4) qk_norm_rotary_kernel(const __grid_con
 
 // Backward.  The CTAs of a side walk over its (token, share of heads) items; every lane sums its 8 columns'
 // g * xhat in fp32, the CTA joins its rows in a fixed order and leaves one partial row of dw, and the
-// kernel below adds those up, also in a fixed order.
+// kernel below adds those up, also in a fixed order.  The next rows' loads (of the same token or the warp's next) are
+// in flight during these rows' arithmetic.  Measured at 9216 tokens of 96 heads of 128 in bf16: 110 us (6.0 TB/s)
+// with three rows ahead and two CTAs on an SM; without loads ahead 129 to 154, with more CTAs and fewer registers
+// 145 to 169 (spills).
 __host__ __device__ constexpr int bwd_unroll(int dtype) { return dtype == QLIN_F32 ? 2 : 3; }
 constexpr int kBwdCtas = 2;  // resident on an SM: 128 registers a thread
 template <int DT, int G, bool kInter>
