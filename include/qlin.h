@@ -325,7 +325,8 @@ int qlin_quantize_rows_fp8(const void* x, int x_dtype, int64_t m, int64_t k, int
  * reference (its hosts run them as separate framework ops around the quantized linears).
  *
  * qlin_rotary_table: positions [tokens, axes] (f32, i32 or i64); axis a turns axes_dim[a] / 2 pairs (host
- * array, even numbers, at most 256 pairs in all), pair i of it by positions[., a] * theta^(-2 i / axes_dim[a]).
+ * array, even numbers, at most 256 pairs in all), pair i of it by positions[., a] * theta^(-2 i / axes_dim[a]),
+ * theta at least 1.
  * table fp32 [tokens, pairs, 2]: (cos, sin), the axes' pairs one after the other.  The angle is formed
  * in 64-bit fractions of a turn, so the table is right to fp32 rounding at any position.
  *

@@ -26,7 +26,7 @@ _Strides = ctypes.c_int64 * 3
 def rotary_table(positions, axes_dim, theta=10000.0):
     """fp32 [..., sum(axes_dim) / 2, 2], (cos, sin) of each pair's angle: positions [..., A] (float32, int32 or
     int64) holds a coordinate per axis, axis a turns axes_dim[a] / 2 pairs, pair i of it by
-    positions[..., a] * theta ** (-2 i / axes_dim[a])."""
+    positions[..., a] * theta ** (-2 i / axes_dim[a]); theta is at least 1."""
     out = native.rotary_table(positions, axes_dim, float(theta))
     if out is not None:
         return out
