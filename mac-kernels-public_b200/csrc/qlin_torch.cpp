@@ -1,8 +1,8 @@
 // qlin._native: the call path of the small operators from torch tensors to the C ABI (include/qlin.h).
 //
 // A call of a few microseconds on the GPU is dominated by what the host does for it, so the checks, the
-// allocation of the outputs and the launch of such operators run here instead of in Python (measured: 6 to 9 us a
-// call against 19 to 50 through ctypes).  These functions take the calls that need nothing else (tensors on
+// allocation of the outputs and the launch of such operators run here instead of in Python (measured: 4 to 8 us a
+// call against 17 to 52 through ctypes).  These functions take the calls that need nothing else (tensors on
 // the current device, whose layout the library reads as it is) and return None for every other one; the Python
 // functions of the same names then copy, convert, switch devices or refuse.  The library's functions are given by
 // address, so that the build that QLIN_LIB selects is the one that runs.
