@@ -45,7 +45,7 @@ __device__ __forceinline__ uint4 aligned_word(const uint8_t* at, int w, const ui
                                               const uint8_t* end) {
   const uint8_t* from = reinterpret_cast<const uint8_t*>(reinterpret_cast<uintptr_t>(at) & ~uintptr_t(15)) + w * 16;
   if (from >= row_end) return uint4{};
-  if (from >= base && from + 16 <= end) return __ldg(reinterpret_cast<const uint4*>(from));
+  if (from >= base && from + 16 <= end) return *reinterpret_cast<const uint4*>(from);
   uint32_t o[4] = {};
 #pragma unroll
   for (int j = 0; j < 16 / kBytes; ++j) {

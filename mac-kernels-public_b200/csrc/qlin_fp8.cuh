@@ -96,6 +96,13 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
   return v;
 }
 
+// An ordinary load, volatile so that it stays where it is written: behind griddep_wait, and ahead of its use.
+__device__ __forceinline__ float ld_f32(const float* p) {
+  float v;
+  asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  return v;
+}
+
 // (a0, a1) += s * (p0, p1)
 __device__ __forceinline__ void ffma2(float s, uint32_t p0, uint32_t p1, float& a0, float& a1) {
   asm("{\n\t.reg .b64 f, sc, acc;\n\t"
@@ -360,14 +367,14 @@ fp8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constan
       const float* sx_next = p.sx + (long long)b_begin * p.ld_sx + min(m, p.M - 1);
       int left = b_end - b_begin - 1;  // blocks after the one sx_next points at
       auto take_sx = [&]() {
-        const float v = qchk(BS_FP8_SCALE, sx_next - p.sx, p.lim_sx) ? __ldg(sx_next) : 0.f;
+        const float v = qchk(BS_FP8_SCALE, sx_next - p.sx, p.lim_sx) ? ld_f32(sx_next) : 0.f;
         if (left > 0) sx_next += p.ld_sx;
         --left;
         return v;
       };
       auto take_sw = [&](int b) {
         const long long i = sw_off + (long long)min(b_begin + b + lane, p.kb - 1) * p.sw_red;
-        return qchk(BS_FP8_SCALE, i, p.lim_sw) ? __ldg(p.sw + i) : 0.f;
+        return qchk(BS_FP8_SCALE, i, p.lim_sw) ? ld_f32(p.sw + i) : 0.f;
       };
       float sx[kAhead], sw = p.kb > 0 ? take_sw(0) : 0.f;  // b counts from b_begin here
       const int blocks = b_end - b_begin;

@@ -22,8 +22,8 @@ __device__ __forceinline__ Raw8<DT> load_raw8(const void* x, long long i) {
   Raw8<DT> r;
   constexpr int kBytes = DT == QLIN_F32 ? 4 : 2;
   const uint4* p = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(x) + i * kBytes);
-  r.v[0] = __ldg(p);
-  if constexpr (DT == QLIN_F32) r.v[1] = __ldg(p + 1);
+  r.v[0] = p[0];
+  if constexpr (DT == QLIN_F32) r.v[1] = p[1];
   return r;
 }
 
@@ -43,7 +43,7 @@ struct Around8 {
     const bool inside = from >= begin && from + kWords * 4 <= begin + lim * kBytes;
     off = inside ? (uint32_t)(at & 15) : 16;
 #pragma unroll
-    for (int j = 0; j < kWords / 4; ++j) v[j] = inside ? __ldg(reinterpret_cast<const uint4*>(from) + j) : uint4{};
+    for (int j = 0; j < kWords / 4; ++j) v[j] = inside ? reinterpret_cast<const uint4*>(from)[j] : uint4{};
     if (!inside) {
       uint32_t o[kWords] = {};
       for (int j = 0; j < 8; ++j) {

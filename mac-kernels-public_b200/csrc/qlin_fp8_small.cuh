@@ -258,7 +258,7 @@ fp8_small_kernel(const __grid_constant__ CUtensorMap tmap_w, const Fp8SmallParam
     const long long sw_off = (long long)nt * p.sw_out;
     auto load_sw = [&](int i) {
       const long long at = sw_off + (long long)(b_begin + min(i, blocks - 1)) * p.sw_red;
-      return qchk(BS_FP8_SCALE, at, p.lim_sw) ? __ldg(p.sw + at) : 0.f;
+      return qchk(BS_FP8_SCALE, at, p.lim_sw) ? p.sw[at] : 0.f;
     };
     float w_next = blocks > 0 ? load_sw(0) : 0.f;
     for (int i = 0; i < blocks; ++i) {

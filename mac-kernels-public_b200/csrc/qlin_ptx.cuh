@@ -221,6 +221,8 @@ __device__ __forceinline__ void fence_proxy_async_smem() {
 }
 // Programmatic dependent launch: the next kernel on the stream, if it was launched for it, may be set up from
 // here on; and a kernel so launched waits until the one before it has completed.  Without it, both do nothing.
+// Such a kernel is resident while earlier work still writes its inputs, so it reads them with ordinary loads behind the
+// wait: the read-only path (__ldg) is for memory that does not change while a kernel lives.
 __device__ __forceinline__ void griddep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // Registers of a thread from here on, for whole warpgroups; an increase waits until others released them.

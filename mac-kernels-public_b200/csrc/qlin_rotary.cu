@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(256) rotary_table_kernel(const __grid_constant
     POS x[kTokens];
 #pragma unroll
     for (int u = 0; u < kTokens; ++u) {
-      x[u] = (u * step < left && qchk(BS_ROT_IN, from - pos, p.tokens * p.axes)) ? __ldg(from) : POS(0);
+      x[u] = (u * step < left && qchk(BS_ROT_IN, from - pos, p.tokens * p.axes)) ? *from : POS(0);
       from += from_step;
     }
 #pragma unroll
@@ -185,19 +185,19 @@ template <int DT, bool kInter>
 __device__ __forceinline__ Pieces<DT> load_pieces(const void* x, long long row, int o0, int o1) {
   Pieces<DT> r;
   if constexpr (DT == QLIN_F32) {
-    const uint4 a = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(x) + row + o0));
-    const uint4 b = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(x) + row + o1));
+    const uint4 a = *reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(x) + row + o0);
+    const uint4 b = *reinterpret_cast<const uint4*>(reinterpret_cast<const float*>(x) + row + o1);
     r.v[0] = make_uint2(a.x, a.y);
     r.v[1] = make_uint2(a.z, a.w);
     r.v[2] = make_uint2(b.x, b.y);
     r.v[3] = make_uint2(b.z, b.w);
   } else if constexpr (kInter) {
-    const uint4 a = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(x) + row + o0));
+    const uint4 a = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(x) + row + o0);
     r.v[0] = make_uint2(a.x, a.y);
     r.v[1] = make_uint2(a.z, a.w);
   } else {
-    r.v[0] = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(x) + row + o0));
-    r.v[1] = __ldg(reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(x) + row + o1));
+    r.v[0] = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(x) + row + o0);
+    r.v[1] = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(x) + row + o1);
   }
   return r;
 }
@@ -288,8 +288,8 @@ struct LanePlan {
 __device__ __forceinline__ void load_turn(const HeadParams& p, long long token_row, int pair0, float (&c)[4],
                                           float (&s)[4]) {
   if (pair0 >= 0 && qchk_span(BS_ROT_IN, token_row + pair0, 4, p.lim_table)) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p.table + token_row + pair0));
-    const float4 b = __ldg(reinterpret_cast<const float4*>(p.table + token_row + pair0) + 1);
+    const float4 a = reinterpret_cast<const float4*>(p.table + token_row + pair0)[0];
+    const float4 b = reinterpret_cast<const float4*>(p.table + token_row + pair0)[1];
     c[0] = a.x; s[0] = a.y; c[1] = a.z; s[1] = a.w;
     c[2] = b.x; s[2] = b.y; c[3] = b.z; s[3] = b.w;
   } else {
@@ -609,7 +609,7 @@ __global__ void __launch_bounds__(256) qk_norm_rotary_any_kernel(const __grid_co
       ga = dy_at(a);
       gb = a == bb ? 0.f : dy_at(bb);
       if (i < p.pairs && qchk(BS_ROT_IN, tr + i, p.lim_table)) {
-        const float2 t = __ldg(p.table + tr + i);
+        const float2 t = p.table[tr + i];
         const float v = ga * t.x + gb * t.y;
         gb = gb * t.x - ga * t.y;
         ga = v;
@@ -645,7 +645,7 @@ __global__ void __launch_bounds__(256) qk_norm_rotary_any_kernel(const __grid_co
       } else {
         const float va = xa * rstd * wa, vb = xb * rstd * wb;
         float2 t = make_float2(1.f, 0.f);
-        if (i < p.pairs && qchk(BS_ROT_IN, tr + i, p.lim_table)) t = __ldg(p.table + tr + i);
+        if (i < p.pairs && qchk(BS_ROT_IN, tr + i, p.lim_table)) t = p.table[tr + i];
         put(a, va * t.x - vb * t.y);
         if (a != bb) put(bb, va * t.y + vb * t.x);
       }
