@@ -25,6 +25,8 @@ def _weight(what, qdata, scale):
     """(qdata with aligned contiguous rows, scale fp32 with a unit inner stride) of a checked weight."""
     if not qdata.is_cuda or not scale.is_cuda:
         raise NotImplementedError("qlin runs on CUDA tensors only (there is no CPU path)")
+    if scale.device != qdata.device:
+        raise ValueError(f"{what}: weight on {qdata.device}, scale on {scale.device}")
     if qdata.dtype != torch.float8_e4m3fn or qdata.dim() != 2:
         raise QlinDecline(1, f"{what}: qdata must be a 2-D float8_e4m3fn tensor")
     n, k = qdata.shape
