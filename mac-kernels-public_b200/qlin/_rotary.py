@@ -96,6 +96,17 @@ def _table(what, q, table):
     return table, table.stride(0) if b > 1 else 0, pairs
 
 
+def _overlaps_itself(x):
+    """Whether rows of x [B, L, H, D] share memory, by the strides from the smallest on (layouts whose rows interleave
+    without nesting count as overlapping too)."""
+    extent = x.shape[3]
+    for step, size in sorted((x.stride(i), x.shape[i]) for i in range(3) if x.shape[i] > 1):
+        if step < extent:
+            return True
+        extent += step * (size - 1)
+    return False
+
+
 def _st(x):
     return _Strides(*x.stride()[:3])
 
@@ -105,8 +116,8 @@ def qk_norm_rotary(q, k, q_weight, k_weight, table, eps=1e-6, interleaved=True, 
     pairs turned by the token's table entries, in fp32 with one rounding.  q [B, L, Hq, D] and k [B, L, Hk, D] may be
     views of one projection's output.  `table` from rotary_table, [L, P, 2] or [B, L, P, 2] with 2 P <= D; pair i is
     values (2 i, 2 i + 1), or (i, i + P) where interleaved is false; values past 2 P are normed only.  `out`: two
-    tensors of the inputs' shapes and dtype to write to, e.g. slices of the buffers of a joint attention (they may
-    not overlap the inputs)."""
+    tensors of the inputs' shapes and dtype to write to, e.g. slices of the buffers of a joint attention (their
+    rows may not overlap, nor may they overlap the inputs)."""
     if out is None:
         got = native.qk_norm_rotary(q, k, q_weight, k_weight, table, eps, interleaved)
         if got is not None:
@@ -124,6 +135,8 @@ def qk_norm_rotary(q, k, q_weight, k_weight, table, eps=1e-6, interleaved=True, 
         for o, x in ((qo, q), (ko, k)):
             if o.shape != x.shape or o.dtype != x.dtype or o.device != x.device or (o.numel() and o.stride(3) != 1):
                 raise ValueError(f"{what}: out must have the inputs' shapes, dtype and device and a unit inner stride")
+            if o.numel() and _overlaps_itself(o):
+                raise ValueError(f"{what}: rows of out overlap (strides {list(o.stride())} for {list(o.shape)})")
     if qo.numel() or ko.numel():
         b, l, hq, d = q.shape
         with torch.cuda.device(q.device):

@@ -21,3 +21,32 @@ def test_linear_refuses_a_weight_or_scale_of_another_device(x, w, s):
         qlin.fp8_linear(_on(x, (4, 128), torch.float32), q, sc)
     with pytest.raises(ValueError, match="cuda:1"):
         qlin.fp8_linear_grad_input(_on(x, (4, 256), torch.float32), q, sc)
+
+
+def _out(q, k, out):
+    import qlin
+    table = _on(0, (5, 8, 2), torch.float32)
+    table.contiguous = lambda: table
+    return qlin.qk_norm_rotary(q, k, None, None, table, out=out)
+
+
+@pytest.mark.parametrize("shape,stride", [((2, 5, 3, 16), (0, 48, 16, 1)), ((2, 5, 3, 16), (240, 0, 16, 1)),
+                                          ((2, 5, 3, 16), (240, 48, 0, 1)), ((2, 5, 3, 16), (240, 48, 8, 1)),
+                                          ((2, 5, 3, 16), (200, 48, 16, 1)), ((2, 5, 3, 16), (16, 16, 160, 1))])
+def test_head_norm_refuses_outputs_that_overlap_themselves(shape, stride):
+    def strided(st):
+        t = _on(0, shape, torch.float32)
+        t.stride = lambda i=None: st if i is None else st[i]
+        return t
+    x, plain = _on(0, shape, torch.float32), (240, 48, 16, 1)
+    for out in ((strided(stride), strided(plain)), (strided(plain), strided(stride))):
+        with pytest.raises(ValueError, match="overlap"):
+            _out(x, x, out)
+
+
+def test_slices_of_joint_buffers_do_not_overlap_themselves():
+    from qlin._rotary import _overlaps_itself
+    joint, first = torch.empty(2, 9, 6, 16), torch.empty(2, 6, 9, 16).transpose(1, 2)
+    for t in (joint, joint[:, 4:], joint[:, ::2, 1:3], joint[:1], joint[:, :1], joint[:, :, :1], joint[..., :8], first,
+              first[:, 2:, ::3], joint.transpose(0, 1), torch.empty(1, 1, 1, 16).as_strided((1, 1, 1, 16), (0, 0, 0, 1))):
+        assert not _overlaps_itself(t), t.stride()
