@@ -1,0 +1,52 @@
+"""The package where the native call path's module is missing, was built for something else, or cannot be built."""
+import os
+import shutil
+import subprocess
+import sys
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+PKG = os.path.join(ROOT, "mac-kernels-public_b200")
+
+
+@pytest.fixture
+def package(tmp_path):
+    """A copy of the Python package beside the library itself, without the module."""
+    shutil.copytree(os.path.join(PKG, "qlin"), tmp_path / "qlin", ignore=shutil.ignore_patterns("*.so", "__pycache__"))
+    return tmp_path
+
+
+def _run(package, code):
+    env = dict(os.environ, PYTHONPATH=str(package), QLIN_LIB=os.path.join(PKG, "qlin", "libqlin.so"))
+    r = subprocess.run([sys.executable, "-c", code], env=env, cwd=package, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-3000:]
+    return r.stdout
+
+
+CALLS = """
+import warnings, torch, qlin
+assert qlin.__file__.startswith({where!r}), qlin.__file__
+try:
+    qlin.int8_linear(torch.zeros(2, 16), torch.zeros(4, 16, dtype=torch.int8), torch.ones(4))
+except NotImplementedError:
+    print("int8 answers")
+w = torch.zeros(64, 128).to(torch.float8_e4m3fn)
+with warnings.catch_warnings(record=True) as told:
+    warnings.simplefilter("always")
+    for _ in range(2):
+        for call in (lambda: qlin.fp8_linear(torch.zeros(2, 128), w, torch.ones(1, 1)),
+                     lambda: qlin.rotary_table(torch.zeros(3, 1), [8])):
+            try:
+                call()
+            except NotImplementedError:
+                print("answers")
+told = [str(t.message) for t in told if "_native" in str(t.message)]
+assert len(told) == 1, told
+print(told[0])
+"""
+
+
+def test_package_without_the_module(package):
+    out = _run(package, CALLS.format(where=str(package)))
+    assert "int8 answers" in out and out.count("answers") == 5 and "build.py" in out
