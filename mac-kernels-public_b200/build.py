@@ -7,7 +7,8 @@ and computed shared-memory index, recorded and read back with qlin_bounds_check)
 qlin/libqlin_checked.so, from objects in _build/checks/; select it with QLIN_LIB.
 
 qlin/_native.so, the call path of the small operators from torch tensors to the C ABI, is compiled from
-csrc/qlin_torch.cpp against the installed torch (no device code; it does not link libqlin.so).
+csrc/qlin_torch.cpp against the installed torch (no device code; it does not link libqlin.so).  Without torch it is
+left out.
 
 Each csrc/*.cu is compiled with nvcc for `-gencode arch=compute_100a,code=sm_100a` into
 _build/, then linked into one shared library with the CUDA runtime linked statically, so the
@@ -53,9 +54,14 @@ def compile_one(src, verbose=False, checks=False):
 
 
 def build_native():
-    """qlin/_native.so: a CPython extension on torch's tensors."""
+    """qlin/_native.so: a CPython extension on torch's tensors.  Left out where there is no torch: the C library
+    needs none."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None:
+        print("torch is not installed: qlin/_native.so is not built", file=sys.stderr)
+        return None
     src = os.path.join(CSRC, "qlin_torch.cpp")
-    torch_dir = list(importlib.util.find_spec("torch").submodule_search_locations)[0]
+    torch_dir = list(spec.submodule_search_locations)[0]
     deps = [src, os.path.join(HERE, "..", "include", "qlin.h"), os.path.join(torch_dir, "version.py")]
     if os.path.exists(OUT_NATIVE) and os.path.getmtime(OUT_NATIVE) >= max(os.path.getmtime(d) for d in deps):
         return OUT_NATIVE

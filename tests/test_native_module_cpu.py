@@ -50,3 +50,17 @@ print(told[0])
 def test_package_without_the_module(package):
     out = _run(package, CALLS.format(where=str(package)))
     assert "int8 answers" in out and out.count("answers") == 5 and "build.py" in out
+
+
+def test_library_builds_without_torch(tmp_path, monkeypatch, capsys):
+    """The C library needs no torch: the module is left out with a note where there is none."""
+    import importlib.util
+    spec = importlib.util.spec_from_file_location("qlin_build", os.path.join(PKG, "build.py"))
+    build = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(build)
+    real = importlib.util.find_spec
+    monkeypatch.setattr(importlib.util, "find_spec", lambda name, *a: None if name == "torch" else real(name, *a))
+    monkeypatch.setattr(build, "OUT_NATIVE", str(tmp_path / "_native.so"))
+    monkeypatch.setattr(build, "compile_one", lambda *a, **k: (build.OUT, ""))  # the objects are not what is tested
+    assert build.build() == build.OUT
+    assert not os.path.exists(build.OUT_NATIVE) and "torch" in capsys.readouterr().err
