@@ -18,6 +18,7 @@ import argparse
 import concurrent.futures as cf
 import importlib.util
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -63,17 +64,25 @@ def build_native():
     src = os.path.join(CSRC, "qlin_torch.cpp")
     torch_dir = list(spec.submodule_search_locations)[0]
     deps = [src, os.path.join(HERE, "..", "include", "qlin.h"), os.path.join(torch_dir, "version.py")]
-    if os.path.exists(OUT_NATIVE) and os.path.getmtime(OUT_NATIVE) >= max(os.path.getmtime(d) for d in deps):
+    with open(os.path.join(torch_dir, "version.py")) as f:
+        version = re.search(r"^__version__ = ['\"](.+)['\"]", f.read(), re.M).group(1)
+    built_for = f"torch {version}, {sysconfig.get_config_var('SOABI')}"
+    stamp = os.path.join(BUILD, "native_built_for")
+    if os.path.exists(OUT_NATIVE) and os.path.getmtime(OUT_NATIVE) >= max(os.path.getmtime(d) for d in deps) and \
+            os.path.exists(stamp) and open(stamp).read() == built_for:
         return OUT_NATIVE
     inc, libs = os.path.join(torch_dir, "include"), os.path.join(torch_dir, "lib")
     cuda = os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")
     cmd = [shutil.which("g++") or "c++", "-O2", "-std=c++17", "-fPIC", "-shared", "-I" + inc,
            "-I" + os.path.join(inc, "torch", "csrc", "api", "include"), "-I" + cuda,
-           "-I" + sysconfig.get_paths()["include"], src, "-o", OUT_NATIVE, "-L" + libs, "-ltorch_python", "-ltorch_cpu",
+           "-I" + sysconfig.get_paths()["include"], f'-DQLIN_BUILT_FOR="{built_for}"', src, "-o", OUT_NATIVE, "-L" + libs, "-ltorch_python", "-ltorch_cpu",
            "-lc10", "-lc10_cuda"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed for {src}:\n{r.stdout}\n{r.stderr}")
+    os.makedirs(BUILD, exist_ok=True)
+    with open(stamp, "w") as f:
+        f.write(built_for)
     return OUT_NATIVE
 
 

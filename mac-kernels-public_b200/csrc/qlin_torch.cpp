@@ -316,4 +316,9 @@ PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, methods
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__native() { return PyModule_Create(&module_def); }
+// The torch and Python that it was compiled against, for the importer to compare with its own.
+PyMODINIT_FUNC PyInit__native() {
+  PyObject* m = PyModule_Create(&module_def);
+  if (m != nullptr && PyModule_AddStringConstant(m, "built_for", QLIN_BUILT_FOR) != 0) Py_CLEAR(m);
+  return m;
+}

@@ -1,14 +1,15 @@
 """The native call path (qlin/_native.so, csrc/qlin_torch.cpp), bound to the loaded library.
 
 Its functions take the calls that need no copy, no conversion and no change of device, and return None for every
-other one, which the Python functions of the same names then handle.  Where the module is missing or does not load
-(it is built against one torch), they handle every call: the same kernels, with more host time for each call, and one
+other one, which the Python functions of the same names then handle.  Where the module is missing, or was built for
+another torch or Python, they handle every call: the same kernels, with more host time for each call, and one
 warning at the first.
 """
 import ctypes
+import sysconfig
 import warnings
 
-import torch  # noqa: F401  (the module links against its libraries)
+import torch
 
 from ._lib import check, lib
 
@@ -37,6 +38,9 @@ def _load():
         from . import _native
     except ImportError as e:
         return _Missing(str(e))
+    here = f"torch {torch.__version__}, {sysconfig.get_config_var('SOABI')}"
+    if getattr(_native, "built_for", None) != here:
+        return _Missing(f"built for {getattr(_native, 'built_for', 'an unknown torch')}, this is {here}")
     _native.bind(check, *(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in _BOUND))
     return _native
 

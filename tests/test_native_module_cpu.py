@@ -64,3 +64,17 @@ def test_library_builds_without_torch(tmp_path, monkeypatch, capsys):
     monkeypatch.setattr(build, "compile_one", lambda *a, **k: (build.OUT, ""))  # the objects are not what is tested
     assert build.build() == build.OUT
     assert not os.path.exists(build.OUT_NATIVE) and "torch" in capsys.readouterr().err
+
+
+@pytest.mark.parametrize("line", ["", "built_for = 'torch 1.0.0, cpython-39-x86_64-linux-gnu'"])
+def test_module_built_for_another_torch_is_not_used(package, line):
+    """Structures of another torch's tensors would be read: the module is left alone."""
+    calls = "".join(f"\ndef {f}(*a):\n    raise SystemError('called')\n" for f in ("bind", "fp8_linear", "rotary_table"))
+    (package / "qlin" / "_native.py").write_text(line + "\n" + calls)
+    out = _run(package, CALLS.format(where=str(package)))
+    assert "int8 answers" in out and out.count("answers") == 5 and "this is torch" in out
+
+
+def test_module_that_is_built_is_used():
+    from qlin import _fast
+    assert _fast.native.__name__ == "qlin._native", _fast.native.why
