@@ -61,7 +61,7 @@ def fp8_linear(x, qdata, scale, bias=None, out_dtype=None):
     """y = x . W^T + bias for the weight W = qdata (float8_e4m3fn [N, K]) times `scale` (fp32
     [ceil(N/128), ceil(K/128)], one per block).  x [..., K] in f32, f16 or bf16, quantized per row and block of
     128 columns; K a multiple of 16.  Returns [..., N] in out_dtype (default x's)."""
-    if out_dtype is None:
+    if out_dtype is None or out_dtype == x.dtype:
         y = native.fp8_linear(x, qdata, scale, bias)
         if y is not None:
             return y
@@ -100,7 +100,7 @@ def fp8_linear(x, qdata, scale, bias=None, out_dtype=None):
 def fp8_linear_grad_input(dy, qdata, scale, out_dtype=None):
     """dx = dy . W for the frozen weight of fp8_linear; dy [..., N] float, quantized per row and block of 128 of
     its N columns, returns [..., K] in out_dtype (default dy's).  The weight is read as it is stored."""
-    if out_dtype is None:
+    if out_dtype is None or out_dtype == dy.dtype:
         dx = native.fp8_linear_grad_input(dy, qdata, scale)
         if dx is not None:
             return dx

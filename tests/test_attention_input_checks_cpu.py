@@ -50,3 +50,54 @@ def test_slices_of_joint_buffers_do_not_overlap_themselves():
     for t in (joint, joint[:, 4:], joint[:, ::2, 1:3], joint[:1], joint[:, :1], joint[:, :, :1], joint[..., :8], first,
               first[:, 2:, ::3], joint.transpose(0, 1), torch.empty(1, 1, 1, 16).as_strided((1, 1, 1, 16), (0, 0, 0, 1))):
         assert not _overlaps_itself(t), t.stride()
+
+
+class _Native:
+    """The native path's functions, here on the CPU, with a count of their calls."""
+
+    def __init__(self):
+        self.calls = []
+
+    def fp8_linear(self, x, qdata, scale, bias):
+        self.calls.append("fp8_linear")
+        return (x.float() @ qdata.float().t()).to(x.dtype)
+
+    def fp8_linear_grad_input(self, dy, qdata, scale):
+        self.calls.append("fp8_linear_grad_input")
+        return (dy.float() @ qdata.float()).to(dy.dtype)
+
+    def qk_norm_rotary(self, q, k, *args):
+        return q * 2, k * 3
+
+    def qk_norm_rotary_backward(self, dq, dk, q, k, q_weight, k_weight, *args):
+        return dq * 2, dk * 3, None if q_weight is None else q_weight * 0, None if k_weight is None else k_weight * 0
+
+
+@pytest.fixture
+def native(monkeypatch):
+    from qlin import _fp8, _rotary
+    n = _Native()
+    monkeypatch.setattr(_fp8, "native", n)
+    monkeypatch.setattr(_rotary, "native", n)
+    return n
+
+
+def test_an_output_type_equal_to_the_inputs_takes_the_native_path(native):
+    import qlin
+    x, w, s = torch.randn(3, 128).bfloat16(), torch.randn(64, 128).to(torch.float8_e4m3fn), torch.ones(1, 1)
+    assert qlin.fp8_linear(x, w, s, out_dtype=torch.bfloat16).shape == (3, 64)
+    assert qlin.fp8_linear_grad_input(x[:, :64], w, s, out_dtype=torch.bfloat16).shape == (3, 128)
+    assert native.calls == ["fp8_linear", "fp8_linear_grad_input"]
+    with pytest.raises(NotImplementedError):  # another type is the general path's
+        qlin.fp8_linear(x, w, s, out_dtype=torch.float32)
+    assert len(native.calls) == 2
+
+
+def test_training_takes_the_native_path_in_both_directions(native):
+    import qlin
+    x = torch.randn(3, 128).bfloat16().requires_grad_(True)
+    w = torch.randn(64, 128).to(torch.float8_e4m3fn)
+    y = qlin.fp8_linear_trainable(x, w, torch.ones(1, 1))
+    y.backward(torch.ones_like(y))
+    assert native.calls == ["fp8_linear", "fp8_linear_grad_input"]
+    assert torch.equal(x.grad, w.float().sum(0).bfloat16().expand(3, 128))
