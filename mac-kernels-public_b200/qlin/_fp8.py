@@ -13,6 +13,7 @@ reference has no 8-bit floating point format; names and argument order follow it
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from ._fast import native
 from ._lib import QlinDecline, check, lib
@@ -164,6 +165,7 @@ class _Fp8Trainable(torch.autograd.Function):
         return fp8_linear(x, qdata, scale, bias)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, gy):
         qdata, scale = ctx.saved_tensors
         gx = gb = None

@@ -14,6 +14,7 @@ from __future__ import annotations
 import ctypes
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from ._fast import native
 from ._lib import QlinDecline, check, lib
@@ -191,6 +192,7 @@ class _QkNormRotary(torch.autograd.Function):
         return qk_norm_rotary(q, k, q_weight, k_weight, table, eps, interleaved)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dq, dk):
         q, k, q_weight, k_weight, table = ctx.saved_tensors
         need = ctx.needs_input_grad

@@ -60,17 +60,17 @@ class _Native:
 
     def fp8_linear(self, x, qdata, scale, bias):
         self.calls.append("fp8_linear")
-        return (x.float() @ qdata.float().t()).to(x.dtype)
+        return (x.float() @ qdata.float().t()).to(x.dtype).detach()
 
     def fp8_linear_grad_input(self, dy, qdata, scale):
         self.calls.append("fp8_linear_grad_input")
-        return (dy.float() @ qdata.float()).to(dy.dtype)
+        return (dy.float() @ qdata.float()).to(dy.dtype).detach()
 
     def qk_norm_rotary(self, q, k, *args):
-        return q * 2, k * 3
+        return (q * 2).detach(), (k * 3).detach()
 
     def qk_norm_rotary_backward(self, dq, dk, q, k, q_weight, k_weight, *args):
-        return dq * 2, dk * 3, None if q_weight is None else q_weight * 0, None if k_weight is None else k_weight * 0
+        return (dq * 2).detach(), (dk * 3).detach(), q_weight.detach() * 0, k_weight.detach() * 0
 
 
 @pytest.fixture
@@ -101,3 +101,25 @@ def test_training_takes_the_native_path_in_both_directions(native):
     y.backward(torch.ones_like(y))
     assert native.calls == ["fp8_linear", "fp8_linear_grad_input"]
     assert torch.equal(x.grad, w.float().sum(0).bfloat16().expand(3, 128))
+
+
+def test_gradients_of_gradients_are_refused(native):
+    """The gradients are the kernels', without a graph: a penalty on them would be left out of the loss unseen."""
+    import qlin
+    x = torch.randn(3, 128, requires_grad=True)
+    w = torch.randn(64, 128).to(torch.float8_e4m3fn)
+    loss = qlin.fp8_linear_trainable(x, w, torch.ones(1, 1)).square().sum()
+    (gx,) = torch.autograd.grad(loss, x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        (loss + gx.square().sum()).backward()
+    q, k = (torch.randn(1, 2, 1, 8, requires_grad=True) for _ in range(2))
+    qw, kw = torch.ones(8, requires_grad=True), torch.ones(8, requires_grad=True)
+    a, b = qlin.qk_norm_rotary_trainable(q, k, qw, kw, torch.zeros(2, 4, 2))
+    loss = a.square().sum() + b.square().sum()
+    (gq,) = torch.autograd.grad(loss, q, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        (loss + gq.square().sum()).backward()
+    # the first derivatives stay what they are
+    loss = qlin.fp8_linear_trainable(x, w, torch.ones(1, 1)).sum()
+    loss.backward()
+    assert torch.equal(x.grad, w.float().sum(0).expand(3, 128))
