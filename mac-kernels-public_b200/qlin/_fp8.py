@@ -12,6 +12,8 @@ reference has no 8-bit floating point format; names and argument order follow it
 """
 from __future__ import annotations
 
+import math
+
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -172,7 +174,7 @@ class _Fp8Trainable(torch.autograd.Function):
         if ctx.needs_input_grad[0]:
             gx = fp8_linear_grad_input(gy, qdata, scale, out_dtype=ctx.x_dtype)
         if ctx.bias is not None and ctx.needs_input_grad[3]:
-            gb = gy.reshape(-1, gy.shape[-1]).float().sum(0).to(ctx.bias[0]).reshape(ctx.bias[1])
+            gb = gy.reshape(math.prod(gy.shape[:-1]), gy.shape[-1]).float().sum(0).to(ctx.bias[0]).reshape(ctx.bias[1])
         return gx, None, None, gb
 
 

@@ -123,3 +123,14 @@ def test_gradients_of_gradients_are_refused(native):
     loss = qlin.fp8_linear_trainable(x, w, torch.ones(1, 1)).sum()
     loss.backward()
     assert torch.equal(x.grad, w.float().sum(0).expand(3, 128))
+
+
+@pytest.mark.parametrize("shape,n", [((3, 128), 0), ((0, 128), 64), ((2, 0, 128), 64), ((128,), 64), ((2, 3, 128), 64)])
+def test_bias_gradient_of_any_shape(native, shape, n):
+    import qlin
+    x, w = torch.randn(shape, requires_grad=True), torch.randn(n, 128).to(torch.float8_e4m3fn)
+    b = torch.zeros(n, requires_grad=True)
+    y = qlin.fp8_linear_trainable(x, w, torch.ones(-(-n // 128), 1), b)
+    y.backward(torch.ones_like(y))
+    rows = y.numel() // n if n else 0
+    assert torch.equal(b.grad, torch.full((n,), float(rows))) and x.grad.shape == shape
