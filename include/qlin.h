@@ -328,7 +328,8 @@ int qlin_quantize_rows_fp8(const void* x, int x_dtype, int64_t m, int64_t k, int
  * array, even numbers, at most 256 pairs in all), pair i of it by positions[., a] * theta^(-2 i / axes_dim[a]),
  * theta at least 1.
  * table fp32 [tokens, pairs, 2]: (cos, sin), the axes' pairs one after the other.  The angle is formed
- * in 64-bit fractions of a turn, so the table is right to fp32 rounding at any position.
+ * in 64-bit fractions of a turn: off by at most |position| * 2^-61 of a turn (2^-57 for theta below 10^4), less than
+ * fp32 rounding up to positions of 2^32 (2^28).
  *
  * qlin_qk_norm_rotary: for each head's row x of head_dim values, v = x * (mean(x^2) + eps)^-1/2 * weight, then
  * pair i turned by the token's table entry: values (2i, 2i + 1) if interleaved, else (i, i + pairs); values
