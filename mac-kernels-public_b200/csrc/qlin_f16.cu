@@ -70,6 +70,22 @@ static PFN_encodeTiled_t encode_fn() {
   return fn;
 }
 
+// The encoder needs a current context.  A thread that has not used CUDA yet (autograd's, a server's) has none until a
+// runtime call binds its device's.
+static CUresult encode_tiled(PFN_encodeTiled_t fn, CUtensorMap* map, CUtensorMapDataType dt, cuuint32_t rank,
+                             const void* base, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box,
+                             const cuuint32_t* estr, CUtensorMapSwizzle swz) {
+  const auto call = [&] {
+    return fn(map, dt, rank, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  const CUresult r = call();
+  int dev = 0;
+  if (r != CUDA_ERROR_INVALID_CONTEXT || cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess)
+    return r;
+  return call();
+}
+
 // 2-D tile map over a row-major matrix [rows, cols] of `elem` bytes with row pitch `pitch_bytes`.
 int make_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dt, int elem, uint64_t cols, uint64_t rows,
                  uint64_t pitch_bytes, uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle swz) {
@@ -88,8 +104,7 @@ int make_tmap_2d(CUtensorMap* map, const void* base, CUtensorMapDataType dt, int
   cuuint32_t box[2] = {box_cols, box_rows};
   cuuint32_t estr[2] = {1, 1};
   (void)elem;
-  CUresult r = fn(map, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  CUresult r = encode_tiled(fn, map, dt, 2, base, dims, strides, box, estr, swz);
   if (r != CUDA_SUCCESS) {
     set_error("cuTensorMapEncodeTiled failed (%d): cols %llu rows %llu pitch %llu box %u x %u", (int)r,
               (unsigned long long)cols, (unsigned long long)rows, (unsigned long long)pitch_bytes, box_cols, box_rows);
@@ -114,8 +129,7 @@ int make_tmap_3d(CUtensorMap* map, const void* base, CUtensorMapDataType dt, int
     set_error("TMA store target needs 16-byte alignment");
     return 1;
   }
-  CUresult r = fn(map, dt, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  CUresult r = encode_tiled(fn, map, dt, 3, base, dims, strides, box, estr, swz);
   if (r != CUDA_SUCCESS) {
     set_error("cuTensorMapEncodeTiled (3-D) failed (%d)", (int)r);
     return 3;
@@ -142,8 +156,7 @@ int make_tmap_3d_strided(CUtensorMap* map, const void* base, CUtensorMapDataType
   cuuint64_t strides[2] = {stride1_bytes, stride2_bytes};
   cuuint32_t box[3] = {b0, b1, 1};
   cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = fn(map, dt, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  CUresult r = encode_tiled(fn, map, dt, 3, base, dims, strides, box, estr, swz);
   if (r != CUDA_SUCCESS) {
     set_error("cuTensorMapEncodeTiled (3-D) failed (%d): %llu x %llu x %llu", (int)r, (unsigned long long)d0,
               (unsigned long long)d1, (unsigned long long)d2);
