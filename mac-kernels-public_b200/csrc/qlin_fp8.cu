@@ -24,7 +24,8 @@ namespace qlin {
 // to a lane, with all its loads issued before the first reduction; the 8 scales of a block, which lie
 // side by side in the block-major scale array, go out as one 32-byte piece.  Values stay as they are stored until
 // they are scaled: four CTAs on an SM in 16 bits.  Measured: 4608 x 16384 bf16 in 37 us (6.1 TB/s read and
-// written), 4608 x 6144 in 17; rows off 16-byte boundaries, 7993 x 4565 bf16, 27 us (4.0 TB/s).
+// written), 4608 x 6144 in 17; rows off 16-byte boundaries, 7993 x 4565 bf16, 27 us (4.1 TB/s), where 7993 x 4568 on
+// them takes 21: a row's words are shifted to their places with nine shuffles instead of one.
 // ---------------------------------------------------------------------------------------------
 struct QuantFp8Params {
   const void* x;

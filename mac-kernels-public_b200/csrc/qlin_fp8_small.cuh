@@ -11,8 +11,10 @@
 // Every block's products have a TMEM buffer of their own, as in the large kernel; a thread owns one channel,
 // each token's scale comes from shared memory.
 //
-// Measured: 2 x 5120 -> 30720 in 27.3 us, 5.8 TB/s of weights (88% of a copy's rate; two CTAs of six 18 KB stages
-// on an SM keep it busy), one token 256 -> 5120 in 3.9 us, of which the products are the smallest part.
+// Measured: 2 x 5120 -> 30720 in 27.2 us, 5.8 TB/s of weights (88% of a copy's rate; two CTAs of six 18 KB stages
+// on an SM keep it busy), one token 256 -> 5120 in 3.8 us, of which the products are the smallest part.  Sixteen tokens
+// 5120 -> 30720 take 30 us in 16 bits and 51 in fp32, whose quantizers hold twice the bytes: 28 of a thread's spill at
+// the 80 registers that two CTAs on an SM leave.
 //
 // Warp roles (384 threads, one tile to a CTA):
 //   warp 0       weight stream (TMA)       warp 1   TMEM alloc + MMA issuer
